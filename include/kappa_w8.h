@@ -208,6 +208,31 @@ int kw8_embed_gather(const int32_t* tokens, int64_t n, kw8_weight table, int64_t
 int kw8_rms_norm(const void* x, int64_t T, int64_t D, const void* scale, int32_t scale_dtype,
                  int32_t kind, float eps, void* out, kw8_stream_t stream);
 
+/* The residual's addition in front of rms_norm, and its result as bf16 rows
+ * or as 8-bit rows for kw8_linear_q8 (kappa keeps the residual stream in
+ * bf16 and norms it as kept: gemma3/block.py:73-82, qwen3/block.py:68-81).
+ *   h = bf16(f32(x) + f32(residual)), or x when residual is NULL;
+ *   y = (f32(h) * rsqrt(mean(f32(h)^2) + eps)) * g            in fp32;
+ *   y_out given: y_out = bf16(y);
+ *   q_out and q_scale_out given: per row s = max(max|y| / 127, FLT_MIN),
+ *     q = round_half_even(y * (1 / s)) in [-127, 127]; a row of y that is
+ *     not finite gets q = 0 and s = NaN.
+ * Squares are summed in fp32, as in kw8_rms_norm: values beyond about 1e19
+ * (or, with eps = 0, below 1e-23) leave that range.
+ * Exactly one of the two results is written; h_out (NULL: not stored) may
+ * be x or residual itself, every other overlap is refused.
+ *   x, residual, h_out, y_out: [T][D] bf16, 16-byte aligned; q_out [T][D]
+ *   int8, 8-byte aligned; q_scale_out [T] fp32; D as for kw8_rms_norm.      */
+int kw8_add_rms_norm(const void* x, const void* residual, int64_t T, int64_t D, const void* scale,
+                     int32_t scale_dtype, int32_t kind, float eps, void* h_out, void* y_out,
+                     int8_t* q_out, float* q_scale_out, kw8_stream_t stream);
+
+/* The values that 8-bit rows (kw8_add_rms_norm) stand for:
+ * out[t][d] = f32(q[t][d]) * scale[t], rounded once to out_dtype; q [T][D]
+ * int8, scale [T] fp32, out [T][D].                                         */
+int kw8_dequantize_rows(const int8_t* q, const float* scale, int64_t T, int64_t D, int32_t out_dtype,
+                        void* out, kw8_stream_t stream);
+
 /* The norms around a decoder block's FFN.  pre_scale [D] (required) is the
  * pre-FFN RMSNorm; post_scale [D] (or NULL: none, as in Qwen3) the post-FFN
  * RMSNorm; both in scale_dtype, of one kind.                                */

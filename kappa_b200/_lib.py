@@ -7,6 +7,7 @@ missing, or no CUDA device is present, calls raise.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -143,6 +144,11 @@ SIGNATURES: dict[str, tuple] = {
     "kw8_linear": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i64, KW8Weight, _i32, _vp, _vp, _sz, _vp]),
     "kw8_embed_gather": (ctypes.c_int, [_vp, _i64, KW8Weight, _i64, _i64, _i32, _vp, _vp]),
     "kw8_rms_norm": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i32, _i32, ctypes.c_float, _vp, _vp]),
+    "kw8_add_rms_norm": (
+        ctypes.c_int,
+        [_vp, _vp, _i64, _i64, _vp, _i32, _i32, ctypes.c_float, _vp, _vp, _vp, _vp, _vp],
+    ),
+    "kw8_dequantize_rows": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i32, _vp, _vp]),
     "kw8_dense_block_workspace_size": (_sz, [_i64, _i64, _i64]),
     "kw8_dense_block": (
         ctypes.c_int,
@@ -247,9 +253,25 @@ def check(rc: int) -> None:
     raise KW8Error(rc, msg)
 
 
+# The handle alone: a torch.cuda.Stream object around it costs 2 us a call.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream
+)
+
+
 def stream_of(t: torch.Tensor) -> int:
     """Handle of torch's current stream on ``t``'s device."""
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return _raw_stream(t.device.index)
+
+
+def on_device(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one (kernels launch on the current device)."""
+    if t.device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(t.device)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def device_status(t: torch.Tensor) -> int:

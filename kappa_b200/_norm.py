@@ -1,10 +1,11 @@
-"""RMSNorm and the fused FFN sub-block shared by the Gemma3 and Qwen3 drop-ins."""
+"""RMSNorm (with the residual's addition, and 8-bit rows) and the fused FFN sub-block shared by the Gemma3 and Qwen3 drop-ins."""
 
 from __future__ import annotations
 
 import torch
 
 from kappa_b200 import _lib
+from kappa_b200.qwen3.quant import Q8Rows
 
 _SCALE_DT = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16}
 
@@ -32,6 +33,52 @@ def rms_norm(x: torch.Tensor, scale: torch.Tensor, *, kind: int, epsilon: float,
     _lib.check(_lib.load().kw8_rms_norm(xc.data_ptr(), T, d, s.data_ptr(), _SCALE_DT[s.dtype], kind,
                                         float(epsilon), out.data_ptr(), _lib.stream_of(x)))
     return out
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, scale: torch.Tensor, *, kind: int, epsilon: float,
+                 quantize: bool):
+    """``kw8_add_rms_norm`` over the last axis: ``(h, y)``, y as bf16 or as ``Q8Rows``.
+
+    ``h`` is ``x`` itself when there is no residual.
+    """
+    _lib.require_cuda(x, "x")
+    if x.dtype != torch.bfloat16:
+        raise ValueError(f"x must be bfloat16 (the W8 path computes in bf16), got {x.dtype}")
+    if x.dim() < 1:
+        raise ValueError("x must have a feature axis")
+    dev = x.device
+    if residual is not None:
+        _lib.require_cuda(residual, "residual")
+        if residual.dtype != torch.bfloat16 or residual.shape != x.shape or residual.device != dev:
+            raise ValueError(f"residual must be bfloat16 {tuple(x.shape)} on {dev}, got {residual.dtype} "
+                             f"{tuple(residual.shape)} on {residual.device}")
+    d = int(x.shape[-1])
+    s = _scale(scale, d, "scale")
+    if s.device != dev:
+        raise ValueError(f"scale is on {s.device}, x on {dev}")
+    lead = x.shape[:-1]
+    with _lib.on_device(x):
+        xc = _rows(x)
+        rc = None if residual is None else _rows(residual)
+        h = x if residual is None else torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
+        y = q = qs = None
+        if quantize:
+            q = torch.empty(x.shape, dtype=torch.int8, device=dev)
+            qs = torch.empty(lead + (1,), dtype=torch.float32, device=dev)
+        else:
+            y = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
+        _lib.check(_lib.load().kw8_add_rms_norm(
+            xc.data_ptr(), None if rc is None else rc.data_ptr(), xc.numel() // d if d else 0, d, s.data_ptr(),
+            _SCALE_DT[s.dtype], kind, float(epsilon), None if rc is None else h.data_ptr(),
+            None if quantize else y.data_ptr(), q.data_ptr() if quantize else None,
+            qs.data_ptr() if quantize else None, _lib.stream_of(x)))
+    return h, (Q8Rows(q, qs) if quantize else y)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and 16-byte aligned (a view that starts elsewhere is copied)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def block_norms(pre: torch.Tensor, post: torch.Tensor | None, d: int, kind: int, epsilon: float):

@@ -963,6 +963,20 @@ int kw8_rms_norm(const void* x, int64_t T, int64_t D, const void* scale, int32_t
   return launch_rms_norm(x, T, D, scale, scale_dtype, kind, eps, out, stream);
 }
 
+int kw8_dequantize_rows(const int8_t* q, const float* scale, int64_t T, int64_t D, int32_t out_dtype, void* out,
+                        kw8_stream_t stream) {
+  KW8_API_BEGIN
+  return launch_dequantize_rows(q, scale, T, D, out_dtype, out, stream);
+}
+
+int kw8_add_rms_norm(const void* x, const void* residual, int64_t T, int64_t D, const void* scale,
+                     int32_t scale_dtype, int32_t kind, float eps, void* h_out, void* y_out, int8_t* q_out,
+                     float* q_scale_out, kw8_stream_t stream) {
+  KW8_API_BEGIN
+  return launch_add_rms_norm(x, residual, T, D, scale, scale_dtype, kind, eps, h_out, y_out, q_out, q_scale_out,
+                             stream);
+}
+
 size_t kw8_dense_block_workspace_size(int64_t T, int64_t D, int64_t H) {
   Carver c(nullptr, SIZE_MAX);
   c.take<__nv_bfloat16>(T * D);

@@ -146,6 +146,123 @@ __global__ void __launch_bounds__(kNormThreads)
   }
 }
 
+// Largest bit pattern over the tpr threads of this thread's row group.
+__device__ __forceinline__ uint32_t group_max(uint32_t v, uint32_t* red, int tpr) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  if (tpr == 32) return v;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) red[warp] = v;  // not the array of group_sum: no barrier needed before
+  __syncthreads();
+  const int wpg = tpr >> 5, first = (warp / wpg) * wpg;
+  for (int w = 0; w < wpg; ++w) v = max(v, red[first + w]);
+  return v;
+}
+
+// Eight gains from d on: g = scale (+ 1 for Gemma).
+__device__ __forceinline__ void load_gain(const void* scale, int dtype, int kind, bool aligned, int64_t d,
+                                          float (&g)[8]) {
+  if (!aligned) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] = load_scale(scale, dtype, d + i);
+  } else if (dtype == KW8_DT_F32) {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(scale) + d);
+    const float4 a = __ldg(p), b = __ldg(p + 1);
+    g[0] = a.x; g[1] = a.y; g[2] = a.z; g[3] = a.w;
+    g[4] = b.x; g[5] = b.y; g[6] = b.z; g[7] = b.w;
+  } else {
+    bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(scale) + d)), g);
+  }
+  if (kind == KW8_NORM_GEMMA)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] += 1.0f;
+}
+
+// Residual add + RMSNorm + optional 8-bit rows (definition in norm.cuh).
+// One pass: a row stays in its threads' registers (kVec 8-wide vectors per
+// thread at most) between the sum of squares, the absmax and the stores, so
+// each input is read once and each output written once; HBM is the bound.
+// The absmax is taken over the bit patterns of |y| (ordered like the values,
+// with infinity and NaN above every number), so one integer reduction also
+// finds the rows that are not finite.  Rounding to int8 is one fma:
+// y * (1/s) + 1.5 * 2^23 leaves the nearest integer (ties to even), in two's
+// complement, in the low byte of the sum's bits.  1/s rounds once, so a
+// value within about 2^-16 of a half step may round to the other side of it
+// than an exact division would.
+template <int kVec, bool kAdd, bool kQ8>
+__global__ void __launch_bounds__(kNormThreads)
+    add_rms_norm_kernel(const uint4* x, const uint4* residual, int64_t T, int64_t D, const void* __restrict__ scale,
+                        int dtype, int kind, bool scale_aligned, float eps, int tpr, uint4* h_out, uint4* y_out,
+                        uint2* q_out, float* s_out) {
+  __shared__ float red[kNormThreads / 32];
+  __shared__ uint32_t red_max[kNormThreads / 32];
+  const int64_t vec = D / 8;
+  const int tl = threadIdx.x % tpr;
+  const int64_t row = blockIdx.x * static_cast<int64_t>(blockDim.x / tpr) + threadIdx.x / tpr;
+  const int nv = row < T ? static_cast<int>((vec - tl + tpr - 1) / tpr) : 0;
+  const int64_t e0 = row * vec + tl;
+  uint4 a[kVec], b[kAdd ? kVec : 1];
+#pragma unroll
+  for (int j = 0; j < kVec; ++j)
+    if (j < nv) {
+      a[j] = x[e0 + j * tpr];
+      if constexpr (kAdd) b[j] = residual[e0 + j * tpr];
+    }
+  float ss = 0.f;
+#pragma unroll
+  for (int j = 0; j < kVec; ++j)
+    if (j < nv) {
+      float f[8];
+      bf16x8_to_f32(a[j], f);
+      if constexpr (kAdd) {
+        float r[8];
+        bf16x8_to_f32(b[j], r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] += r[i];
+        a[j] = f32x8_to_bf16(f);  // the residual stream is kept in bf16, and normed as it is kept
+        bf16x8_to_f32(a[j], f);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
+    }
+  const float total = group_sum(ss, red, tpr);
+  const float r = rsqrtf(__fdiv_rn(total, static_cast<float>(D)) + eps);
+  float v[kVec][8];
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < kVec; ++j)
+    if (j < nv) {
+      if (h_out != nullptr) h_out[e0 + j * tpr] = a[j];
+      float g[8];
+      load_gain(scale, dtype, kind, scale_aligned, (static_cast<int64_t>(j) * tpr + tl) * 8, g);
+      bf16x8_to_f32(a[j], v[j]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[j][i] = __fmul_rn(__fmul_rn(v[j][i], r), g[i]);
+        if constexpr (kQ8) top = max(top, __float_as_uint(v[j][i]) & 0x7FFFFFFFu);
+      }
+      if constexpr (!kQ8) y_out[e0 + j * tpr] = f32x8_to_bf16(v[j]);
+    }
+  if constexpr (kQ8) {
+    top = group_max(top, red_max, tpr);
+    const bool finite = top < 0x7F800000u;
+    const float s = finite ? fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), 1.17549435e-38f)
+                           : __uint_as_float(0x7FC00000u);
+    const float inv = __fdiv_rn(1.0f, s);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j)
+      if (j < nv) {
+        uint32_t m[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m[i] = __float_as_uint(fmaf(v[j][i], inv, 12582912.0f));
+        uint2 o;
+        o.x = __byte_perm(__byte_perm(m[0], m[1], 0x0040), __byte_perm(m[2], m[3], 0x0040), 0x5410);
+        o.y = __byte_perm(__byte_perm(m[4], m[5], 0x0040), __byte_perm(m[6], m[7], 0x0040), 0x5410);
+        q_out[e0 + j * tpr] = finite ? o : make_uint2(0u, 0u);
+      }
+    if (tl == 0 && row < T) s_out[row] = s;
+  }
+}
+
 // Threads per row: the fewest of 32, 64, 128, 256 that hold a row in at most
 // kNormMaxVec vectors each, doubled while the rows would keep fewer than
 // ~131k threads busy (few rows: more threads per row; measured at T = 256 /
@@ -215,6 +332,64 @@ int launch_block_finish(const float* part, int splits, int64_t split_stride, int
       static_cast<const uint4*>(h), tpr, static_cast<uint4*>(out));
   KW8_CHECK_LAUNCH();
   return KW8_OK;
+}
+
+namespace {
+
+template <int kVec>
+int launch_add_rms_norm_vec(const uint4* x, const uint4* residual, int64_t T, int64_t D, const void* scale,
+                            int scale_dtype, int kind, float eps, int tpr, uint4* h_out, uint4* y_out,
+                            uint2* q_out, float* s_out, cudaStream_t stream) {
+  const int64_t rpc = norm_rows_per_cta(T, tpr);
+  const unsigned grid = static_cast<unsigned>((T + rpc - 1) / rpc), block = static_cast<unsigned>(rpc * tpr);
+  const bool aligned = (reinterpret_cast<uintptr_t>(scale) & 15) == 0;
+  auto kernel = residual ? (q_out ? add_rms_norm_kernel<kVec, true, true> : add_rms_norm_kernel<kVec, true, false>)
+                         : (q_out ? add_rms_norm_kernel<kVec, false, true> : add_rms_norm_kernel<kVec, false, false>);
+  kernel<<<grid, block, 0, stream>>>(x, residual, T, D, scale, scale_dtype, kind, aligned, eps, tpr, h_out, y_out,
+                                     q_out, s_out);
+  KW8_CHECK_LAUNCH();
+  return KW8_OK;
+}
+
+bool overlaps(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+  return a && b && p < q + static_cast<uintptr_t>(nb) && q < p + static_cast<uintptr_t>(na);
+}
+
+}  // namespace
+
+int launch_add_rms_norm(const void* x, const void* residual, int64_t T, int64_t D, const void* scale,
+                        int scale_dtype, int kind, float eps, void* h_out, void* y_out, int8_t* q_out,
+                        float* s_out, cudaStream_t stream) {
+  int rc = check_norm(T, D, scale_dtype, kind, eps);
+  if (rc || T == 0) return rc;
+  KW8_REQUIRE(x && scale, KW8_ERR_INVALID_ARG, "null x/scale");
+  KW8_REQUIRE((y_out != nullptr) != (q_out != nullptr) && (q_out != nullptr) == (s_out != nullptr),
+              KW8_ERR_INVALID_ARG, "the norm writes either bf16 rows or int8 rows with their scales");
+  KW8_REQUIRE(((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) |
+                reinterpret_cast<uintptr_t>(h_out) | reinterpret_cast<uintptr_t>(y_out)) & 15) == 0 &&
+                  (reinterpret_cast<uintptr_t>(q_out) & 7) == 0 && (reinterpret_cast<uintptr_t>(s_out) & 3) == 0,
+              KW8_ERR_UNSUPPORTED, "RMSNorm rows must be 16-byte aligned (int8 rows 8-byte)");
+  // Outputs: h over its own input element by element, or no overlap at all.
+  const int64_t n2 = T * D * 2, out_bytes = q_out ? T * D : n2;
+  const void* out = q_out ? static_cast<const void*>(q_out) : y_out;
+  bool bad = overlaps(out, out_bytes, x, n2) || overlaps(out, out_bytes, residual, n2) ||
+             overlaps(out, out_bytes, h_out, n2) || overlaps(s_out, T * 4, out, out_bytes) ||
+             overlaps(s_out, T * 4, h_out, n2) || overlaps(s_out, T * 4, x, n2) || overlaps(s_out, T * 4, residual, n2);
+  for (const void* in : {x, residual}) bad = bad || (h_out != in && overlaps(h_out, n2, in, n2));
+  const int64_t scale_bytes = D * (scale_dtype == KW8_DT_F32 ? 4 : 2);
+  bad = bad || overlaps(scale, scale_bytes, out, out_bytes) || overlaps(scale, scale_bytes, h_out, n2) ||
+        overlaps(scale, scale_bytes, s_out, T * 4);
+  KW8_REQUIRE(!bad, KW8_ERR_INVALID_ARG, "the norm's outputs overlap its inputs or one another");
+  const int tpr = norm_tpr(T, D);
+  const int64_t per = (D / 8 + tpr - 1) / tpr;  // 8-wide vectors per thread
+  auto go = per <= 1 ? launch_add_rms_norm_vec<1>
+                     : per <= 2 ? launch_add_rms_norm_vec<2>
+                                : per <= 4 ? launch_add_rms_norm_vec<4>
+                                           : per <= 5 ? launch_add_rms_norm_vec<5> : launch_add_rms_norm_vec<kNormMaxVec>;
+  return go(static_cast<const uint4*>(x), static_cast<const uint4*>(residual), T, D, scale, scale_dtype, kind, eps,
+            tpr, static_cast<uint4*>(h_out), static_cast<uint4*>(y_out), reinterpret_cast<uint2*>(q_out), s_out,
+            stream);
 }
 
 }  // namespace kw8

@@ -275,4 +275,73 @@ int launch_dequantize(const kw8_weight& w, int64_t groups, int64_t N, int64_t K,
   return KW8_OK;
 }
 
+namespace {
+
+// The values that 8-bit rows stand for.  A warp per row; with 16-byte
+// aligned rows (kVec) a lane reads 16 values at once.  HBM bound: D bytes
+// read and 2 D (4 D) written per row.
+template <bool kVec, bool kF32>
+__global__ void __launch_bounds__(256)
+    dequantize_rows_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale, int64_t T, int64_t D,
+                           void* __restrict__ out) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = blockIdx.x * static_cast<int64_t>(blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (row >= T) return;
+  const float s = __ldg(scale + row);
+  if constexpr (kVec) {
+    const uint4* src = reinterpret_cast<const uint4*>(q + row * D);
+    for (int64_t j = lane; j < D / 16; j += 32) {
+      const uint4 v = __ldg(src + j);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      float f[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f[i] = static_cast<float>(static_cast<int8_t>(w[i / 4] >> (8 * (i % 4)))) * s;
+      if constexpr (kF32) {
+        float4* dst = reinterpret_cast<float4*>(static_cast<float*>(out) + row * D) + j * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dst[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+      } else {
+        uint32_t o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+          o[i] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + row * D) + j * 2;
+        dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+        dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+      }
+    }
+  } else {
+    for (int64_t d = lane; d < D; d += 32) {
+      const float f = static_cast<float>(q[row * D + d]) * s;
+      if constexpr (kF32)
+        static_cast<float*>(out)[row * D + d] = f;
+      else
+        static_cast<__nv_bfloat16*>(out)[row * D + d] = __float2bfloat16_rn(f);
+    }
+  }
+}
+
+}  // namespace
+
+int launch_dequantize_rows(const int8_t* q, const float* scale, int64_t T, int64_t D, int out_dtype, void* out,
+                           cudaStream_t stream) {
+  KW8_REQUIRE(T >= 0 && D >= 0, KW8_ERR_INVALID_ARG, "bad shape (T=%lld D=%lld)", (long long)T, (long long)D);
+  KW8_REQUIRE(out_dtype == KW8_DT_F32 || out_dtype == KW8_DT_BF16, KW8_ERR_INVALID_ARG, "bad out dtype");
+  KW8_REQUIRE(T < (1ll << 31), KW8_ERR_UNSUPPORTED, "too many rows");
+  if (T == 0 || D == 0) return KW8_OK;
+  KW8_REQUIRE(q && scale && out, KW8_ERR_INVALID_ARG, "null pointer");
+  const bool f32 = out_dtype == KW8_DT_F32;
+  KW8_REQUIRE((reinterpret_cast<uintptr_t>(out) & (f32 ? 3 : 1)) == 0 && (reinterpret_cast<uintptr_t>(scale) & 3) == 0,
+              KW8_ERR_UNSUPPORTED, "misaligned rows");
+  const bool vec =
+      D % 16 == 0 && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  auto kernel = vec ? (f32 ? dequantize_rows_kernel<true, true> : dequantize_rows_kernel<true, false>)
+                    : (f32 ? dequantize_rows_kernel<false, true> : dequantize_rows_kernel<false, false>);
+  kernel<<<static_cast<unsigned>((T + 7) / 8), 256, 0, stream>>>(q, scale, T, D, out);
+  KW8_CHECK_LAUNCH();
+  return KW8_OK;
+}
+
 }  // namespace kw8

@@ -15,4 +15,8 @@ int launch_dequantize(const kw8_weight& w, int64_t groups, int64_t N, int64_t K,
 int launch_embed_gather(const int32_t* tokens, int64_t n, const kw8_weight& table, int64_t V,
                         int64_t D, int out_dtype, void* out, cudaStream_t stream);
 
+// out[t][d] = dt(f32(q[t][d]) * scale[t]), rounded once to out_dtype.
+int launch_dequantize_rows(const int8_t* q, const float* scale, int64_t T, int64_t D, int out_dtype, void* out,
+                           cudaStream_t stream);
+
 }  // namespace kw8

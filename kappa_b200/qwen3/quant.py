@@ -24,6 +24,7 @@ from kappa_b200 import _lib
 
 __all__ = [
     "Q8Weight",
+    "Q8Rows",
     "Weight",
     "is_q8_weight",
     "weight_param_dtype",
@@ -31,6 +32,7 @@ __all__ = [
     "quantize_weight",
     "kmajor",
     "gather_embed_tokens",
+    "dequantize_rows",
     "Q8Tiled",
     "pack_weight",
     "unpack_weight",
@@ -45,6 +47,15 @@ class Q8Weight(NamedTuple):
 
 
 Weight: TypeAlias = torch.Tensor | Q8Weight
+
+
+class Q8Rows(NamedTuple):
+    """Activation rows in 8 bits, as ``add_rms_norm_q8`` makes them: int8 ``values``
+    ``[.., D]`` and one fp32 ``scale`` per row ``[.., 1]``; they stand for
+    ``values * scale``.  ``linear_q8`` multiplies them with W8 weights."""
+
+    values: torch.Tensor
+    scale: torch.Tensor
 
 
 def is_q8_weight(w: Weight) -> TypeGuard[Q8Weight]:
@@ -258,6 +269,34 @@ def to_compute_dtype(w: Weight, dtype: torch.dtype, *, in_axis: int = -2) -> tor
             _lib.load().kw8_dequantize(km.struct(), groups, N, K, _DT[dtype], out.data_ptr(), _lib.stream_of(out))
         )
     return out.transpose(-1, -2) if _norm_axis(in_axis, out.dim()) == -2 else out
+
+
+def check_rows(x: Q8Rows, name: str = "x") -> None:
+    """``x`` is a ``Q8Rows`` of CUDA tensors of one device with one scale per row."""
+    v, s = x.values, x.scale
+    _lib.require_cuda(v, name)
+    _lib.require_cuda(s, f"{name}.scale")
+    if v.dtype != torch.int8 or s.dtype != torch.float32:
+        raise ValueError(f"{name}: 8-bit rows are int8 values with fp32 scales, got {v.dtype} and {s.dtype}")
+    if v.dim() < 1 or s.shape != v.shape[:-1] + (1,):
+        raise ValueError(f"{name}: values {tuple(v.shape)} need one scale per row, got {tuple(s.shape)}")
+    if s.device != v.device:
+        raise ValueError(f"{name}: scale and values on different devices")
+
+
+def dequantize_rows(x: Q8Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values that 8-bit rows stand for: ``values * scale`` in fp32, rounded once to ``dtype``."""
+    check_rows(x)
+    if dtype not in _DT:
+        raise ValueError(f"dequantize_rows: unsupported dtype {dtype}")
+    v = x.values
+    d = int(v.shape[-1])
+    with _lib.on_device(v):
+        vc, sc = v.contiguous(), x.scale.contiguous()
+        out = torch.empty(v.shape, dtype=dtype, device=v.device)
+        _lib.check(_lib.load().kw8_dequantize_rows(vc.data_ptr(), sc.data_ptr(), vc.numel() // d if d else 0, d,
+                                                   _DT[dtype], out.data_ptr(), _lib.stream_of(v)))
+    return out
 
 
 def gather_embed_tokens(tokens: torch.Tensor, embed: Weight, *, compute_dtype: torch.dtype) -> torch.Tensor:
