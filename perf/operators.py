@@ -121,23 +121,19 @@ def prepare(case, seed):
     return s
 
 
-def _stands_for(values, scale):
-    """The values that int8 rows stand for, in bf16."""
-    return torch.mul(values, scale, out=torch.empty(values.shape, dtype=torch.bfloat16, device=values.device))
-
-
 def _norm_own(s):
     from kappa_b200.gemma3 import norms as gemma
     from kappa_b200.qwen3 import norms as qwen
+    from kappa_b200.qwen3.quant import dequantize_rows
 
     n = gemma if s["gemma"] else qwen
     if s["out"] == "bf16":
         return n.add_rms_norm(s["x"], s["residual"], s["g"]) if s["residual"] is not None else n.rms_norm(s["x"], s["g"])
     if s["residual"] is None:
         q = n.rms_norm_q8(s["x"], s["g"])
-        return _stands_for(q.values, q.scale), q.scale
+        return dequantize_rows(q), q.scale
     h, q = n.add_rms_norm_q8(s["x"], s["residual"], s["g"])
-    return h, _stands_for(q.values, q.scale), q.scale
+    return h, dequantize_rows(q), q.scale
 
 
 def _norm_plain(s):
