@@ -192,6 +192,17 @@ int kw8_linear(const void* x, const int32_t* rows, int64_t T, int64_t K, int64_t
                kw8_weight w, int32_t out_dtype, void* out, void* workspace,
                size_t workspace_bytes, kw8_stream_t stream);
 
+/* The same layer on 8-bit rows (kw8_add_rms_norm):
+ *   out[t][n] = (Σ_k q[t][k] * w.q[n][k]) * q_scale[t] * s[n].
+ * The sum is exact (int32); one rounding to fp32, the two scale products in
+ * this order, and for bf16 one more rounding.
+ *   q   : int8 [T][K], 16-byte aligned, K % 16 == 0, K <= 131056;
+ *   q_scale: fp32 [T] (a NaN scale makes its row NaN);
+ *   w   : one group, either layout; out: [T][N] in out_dtype.
+ * No workspace; the result does not depend on how the work was split.       */
+int kw8_linear_q8(const int8_t* q, const float* q_scale, int64_t T, int64_t K, int64_t N, kw8_weight w,
+                  int32_t out_dtype, void* out, kw8_stream_t stream);
+
 /* gather_embed_tokens (kappa/qwen3/quant.py:51-57) for a W8 table:
  * out[i][d] = dt(q[v][d]) * dt(s) with v = tokens[i], rounded once to
  * out_dtype, s the table's scale (per tensor, or per row v).  Ids follow a

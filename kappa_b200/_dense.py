@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 
 from kappa_b200 import _lib
-from kappa_b200.qwen3.quant import KMajor
+from kappa_b200.qwen3.quant import KMajor, Q8Rows, check_rows
 
 
 def check_x(x: torch.Tensor, d: int | None = None) -> None:
@@ -87,4 +87,34 @@ def linear(
         )
     )
     del rows_c
+    return out
+
+
+def linear_q8(x: Q8Rows, w: KMajor, *, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``(x.values . w^T) * x.scale`` through ``kw8_linear_q8``: ``[.., K]`` 8-bit rows, ``w`` K-major ``[.., N, K]``.
+
+    Returns ``[.., N]``, N over all leading axes of ``w``.
+    """
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"out_dtype must be bfloat16 or float32, got {out_dtype}")
+    check_rows(x)
+    v = x.values
+    K = int(w.shape[-1])
+    if int(v.shape[-1]) != K:
+        raise ValueError(f"x rows have {int(v.shape[-1])} features, the weight takes {K}")
+    if w.layout == _lib.LAYOUT_TILED and len(w.shape) > 2 and int(w.shape[-2]) % 16:
+        raise ValueError("a stacked tiled weight is one linear layer only when its rows per group are a multiple of 16")
+    if w.q.device != v.device:
+        raise ValueError(f"x is on {v.device}, the weight on {w.q.device}")
+    N = 1
+    for d in w.shape[:-1]:
+        N *= d
+    with _lib.on_device(v):
+        vc, sc = v.contiguous(), x.scale.contiguous()
+        if vc.data_ptr() % 16:
+            vc = vc.clone()
+        out = vc.new_empty(v.shape[:-1] + (N,), dtype=out_dtype)
+        _lib.check(_lib.load().kw8_linear_q8(
+            vc.data_ptr(), sc.data_ptr(), vc.numel() // K, K, N, w.struct(),
+            _lib.DT_F32 if out_dtype == torch.float32 else _lib.DT_BF16, out.data_ptr(), _lib.stream_of(vc)))
     return out

@@ -142,6 +142,7 @@ SIGNATURES: dict[str, tuple] = {
     ),
     "kw8_linear_workspace_size": (_sz, [_i64, _i64, _i64]),
     "kw8_linear": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i64, KW8Weight, _i32, _vp, _vp, _sz, _vp]),
+    "kw8_linear_q8": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i64, KW8Weight, _i32, _vp, _vp]),
     "kw8_embed_gather": (ctypes.c_int, [_vp, _i64, KW8Weight, _i64, _i64, _i32, _vp, _vp]),
     "kw8_rms_norm": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i32, _i32, ctypes.c_float, _vp, _vp]),
     "kw8_add_rms_norm": (

@@ -16,7 +16,7 @@ def _scale(s: torch.Tensor, d: int, name: str) -> torch.Tensor:
         raise ValueError(f"{name}: scale dtype {s.dtype} unsupported")
     if s.numel() != d:
         raise ValueError(f"{name}: {s.numel()} values for {d} features")
-    return s.reshape(d).contiguous()
+    return s if s.dim() == 1 and s.is_contiguous() else s.reshape(d).contiguous()
 
 
 def rms_norm(x: torch.Tensor, scale: torch.Tensor, *, kind: int, epsilon: float,
@@ -56,22 +56,22 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, scale: torch.Te
     s = _scale(scale, d, "scale")
     if s.device != dev:
         raise ValueError(f"scale is on {s.device}, x on {dev}")
-    lead = x.shape[:-1]
     with _lib.on_device(x):
         xc = _rows(x)
         rc = None if residual is None else _rows(residual)
-        h = x if residual is None else torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
+        h = x if rc is None else torch.empty_like(xc)
         y = q = qs = None
         if quantize:
-            q = torch.empty(x.shape, dtype=torch.int8, device=dev)
-            qs = torch.empty(lead + (1,), dtype=torch.float32, device=dev)
+            q = torch.empty_like(xc, dtype=torch.int8)
+            qs = xc.new_empty(xc.shape[:-1] + (1,), dtype=torch.float32)
+            out = (None, q.data_ptr(), qs.data_ptr())
         else:
-            y = torch.empty(x.shape, dtype=torch.bfloat16, device=dev)
+            y = torch.empty_like(xc)
+            out = (y.data_ptr(), None, None)
+        T = xc.numel() // d if d else 0
         _lib.check(_lib.load().kw8_add_rms_norm(
-            xc.data_ptr(), None if rc is None else rc.data_ptr(), xc.numel() // d if d else 0, d, s.data_ptr(),
-            _SCALE_DT[s.dtype], kind, float(epsilon), None if rc is None else h.data_ptr(),
-            None if quantize else y.data_ptr(), q.data_ptr() if quantize else None,
-            qs.data_ptr() if quantize else None, _lib.stream_of(x)))
+            xc.data_ptr(), None if rc is None else rc.data_ptr(), T, d, s.data_ptr(), _SCALE_DT[s.dtype], kind, epsilon,
+            None if rc is None else h.data_ptr(), *out, _lib.stream_of(xc)))
     return h, (Q8Rows(q, qs) if quantize else y)
 
 

@@ -3,6 +3,7 @@
 #include <climits>
 #include <cmath>
 
+#include "gemm_q8.cuh"
 #include "gemm_stream.cuh"
 #include "gemm_tc.cuh"
 #include "moe.cuh"
@@ -946,6 +947,34 @@ int kw8_linear(const void* x, const int32_t* rows, int64_t T, int64_t K, int64_t
   KW8_REQUIRE(workspace != nullptr && c.ok, KW8_ERR_WORKSPACE, "linear workspace too small (%zu < %zu)",
               workspace_bytes, c.off);
   return linear(x, rows, T, K, N, w, out_dtype == KW8_DT_F32, out, b, stream);
+}
+
+int kw8_linear_q8(const int8_t* q, const float* q_scale, int64_t T, int64_t K, int64_t N, kw8_weight w,
+                  int32_t out_dtype, void* out, kw8_stream_t stream) {
+  KW8_API_BEGIN
+  KW8_REQUIRE(T >= 0 && K > 0 && N > 0, KW8_ERR_INVALID_ARG, "bad shape (T=%lld K=%lld N=%lld)", (long long)T,
+              (long long)K, (long long)N);
+  KW8_REQUIRE(out_dtype == KW8_DT_BF16 || out_dtype == KW8_DT_F32, KW8_ERR_INVALID_ARG, "bad out dtype");
+  KW8_REQUIRE(K % 16 == 0 && K <= kQ8MaxK, KW8_ERR_UNSUPPORTED,
+              "K=%lld must be a multiple of 16 up to %lld (int32 sums)", (long long)K, (long long)kQ8MaxK);
+  KW8_REQUIRE(T < (1ll << 31) && N < (1ll << 31) - 256, KW8_ERR_UNSUPPORTED, "shape out of range");
+  int rc = check_weight(w, "weight");
+  if (rc || T == 0) return rc;
+  KW8_REQUIRE(q && q_scale && out, KW8_ERR_INVALID_ARG, "null q/scale/out");
+  const bool f32 = out_dtype == KW8_DT_F32;
+  KW8_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(w.q)) & 15) == 0 &&
+                  (reinterpret_cast<uintptr_t>(q_scale) & 3) == 0 &&
+                  (reinterpret_cast<uintptr_t>(w.scale) & (w.scale_dtype == KW8_DT_F32 ? 3 : 1)) == 0 &&
+                  (reinterpret_cast<uintptr_t>(out) & (f32 ? 3 : 1)) == 0,
+              KW8_ERR_UNSUPPORTED, "int8 operands must be 16-byte aligned, scales and out to their type");
+  Q8LinearArgs a{};
+  a.T = static_cast<int>(T);
+  a.N = static_cast<int>(N);
+  a.K = static_cast<int>(K);
+  a.x_scale = q_scale;
+  a.out = out;
+  a.out_f32 = f32 ? 1 : 0;
+  return launch_linear_q8(q, w, a, stream);
 }
 
 int kw8_embed_gather(const int32_t* tokens, int64_t n, kw8_weight table, int64_t V, int64_t D,

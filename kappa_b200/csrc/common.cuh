@@ -416,6 +416,17 @@ __device__ __forceinline__ uint64_t smem_desc_kmajor_sw128(uint32_t saddr) {
       : "r"(taddr)                                                             \
       : "memory")
 
+#define KW8_TMEM_LD_X16(taddr, v)                                              \
+  asm volatile(                                                                \
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, "   \
+      "%7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"                      \
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]),           \
+        "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),           \
+        "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]),      \
+        "=r"(v[15])                                                            \
+      : "r"(taddr)                                                             \
+      : "memory")
+
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -435,8 +446,8 @@ int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype,
 
 // Tensor map of a pre-packed (tiled) int8 weight with `tile_rows` feature
 // tiles of `steps` 1 KB blocks each, viewed as [tile_rows][steps * 4][256 B];
-// box: 2 steps (one 128-k stage) of `box_tiles` feature tiles.
+// box: `box_steps` steps (two: one 128-k stage) of `box_tiles` feature tiles.
 int make_tmap_tiled(CUtensorMap* map, const void* base, uint64_t tile_rows, uint64_t steps,
-                    uint32_t box_tiles);
+                    uint32_t box_tiles, uint32_t box_steps = 2);
 
 }  // namespace kw8

@@ -7,6 +7,7 @@
 #include "gemm_tc.cu"
 #include "gemm_tc2.cu"
 #include "gemm_stream.cu"
+#include "gemm_q8.cu"
 #include "moe.cu"
 #include "norm.cu"
 #include "api.cu"

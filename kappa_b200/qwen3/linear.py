@@ -10,6 +10,11 @@ head_dim]`` for O (the storage :func:`quantize_attn_out` produces).
 kappa computes ``einsum(x, to_compute_dtype(w, x.dtype))``: a bf16 product
 of bf16 dequantised weights; here the int8 values are widened exactly, the
 products accumulate in fp32 and the scale is applied to the sum.
+
+The projections also take 8-bit rows (``Q8Rows``, made by ``add_rms_norm_q8``)
+in place of bf16 ones, and :func:`linear_q8` is that product for any W8
+weight: int8 x int8 on the tensor core with exact int32 sums
+(``kw8_linear_q8``).
 """
 
 from __future__ import annotations
@@ -17,28 +22,42 @@ from __future__ import annotations
 import torch
 
 from kappa_b200 import _dense
-from kappa_b200.qwen3.quant import KMajor, Q8Weight, Weight, is_q8_weight, kmajor, quantize_weight
+from kappa_b200.qwen3.quant import KMajor, Q8Rows, Q8Weight, Weight, is_q8_weight, kmajor, quantize_weight
 
-__all__ = ["project_q", "project_kv", "project_attn_out", "quantize_attn_out", "attn_out_kmajor"]
+__all__ = ["project_q", "project_kv", "project_attn_out", "quantize_attn_out", "attn_out_kmajor",
+           "linear_q8"]
 
 
-def _project_heads(x: torch.Tensor, w: Weight, name: str) -> torch.Tensor:
+def linear_q8(x: Q8Rows, w: Weight, *, in_axis: int = -1, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """8-bit rows ``[.., K]`` times a W8 weight ``[.., N, K]`` (``in_axis=-1``) or ``[.., K, N]`` (``-2``): ``[.., N]``.
+
+    ``out[t, n] = (sum_k x.values[t, k] * w.values[n, k]) * x.scale[t] * w.scale[n]``; N counts the leading axes of a
+    stacked weight too.
+    """
+    if not isinstance(x, Q8Rows):
+        raise TypeError("x: linear_q8 takes 8-bit rows (add_rms_norm_q8, rms_norm_q8)")
+    return _dense.linear_q8(x, kmajor(w, in_axis, "w"), out_dtype=out_dtype)
+
+
+def _project_heads(x: torch.Tensor | Q8Rows, w: Weight, name: str) -> torch.Tensor:
     """``einsum("btd,ndh->btnh", x, w)`` for a W8 ``w`` ``[n, d, h]``."""
     km = kmajor(w, -2, name)
     if len(km.shape) != 3:
         raise ValueError(f"{name} must be [heads, model_dim, head_dim], got {tuple(w.values.shape)}")
     n, h, d = (int(s) for s in km.shape)
+    if isinstance(x, Q8Rows):
+        return _dense.linear_q8(x, km).unflatten(-1, (n, h))
     _dense.check_x(x, d)
     b, t = int(x.shape[0]), int(x.shape[1])
     return _dense.linear(x.reshape(b * t, d), km).reshape(b, t, n, h)
 
 
-def project_q(x: torch.Tensor, q_w: Weight) -> torch.Tensor:
+def project_q(x: torch.Tensor | Q8Rows, q_w: Weight) -> torch.Tensor:
     """kappa/qwen3/linear.py:11-13: ``q_w`` ``[num_heads, model_dim, head_dim]``."""
     return _project_heads(x, q_w, "q_w")
 
 
-def project_kv(x: torch.Tensor, k_w: Weight, v_w: Weight) -> tuple[torch.Tensor, torch.Tensor]:
+def project_kv(x: torch.Tensor | Q8Rows, k_w: Weight, v_w: Weight) -> tuple[torch.Tensor, torch.Tensor]:
     """kappa/qwen3/linear.py:16-20: ``k_w``, ``v_w`` each ``[num_kv, model_dim, head_dim]``."""
     return _project_heads(x, k_w, "k_w"), _project_heads(x, v_w, "v_w")
 

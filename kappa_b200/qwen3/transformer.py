@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from kappa_b200 import _dense
-from kappa_b200.qwen3.quant import Weight, gather_embed_tokens, is_q8_weight, kmajor
+from kappa_b200.qwen3.quant import Q8Rows, Weight, gather_embed_tokens, is_q8_weight, kmajor
 
 __all__ = ["embed_tokens", "logits_from_hidden", "logits_from_hidden_tied", "logits_from_hidden_last_positions"]
 
@@ -30,12 +30,17 @@ def _head(x: torch.Tensor, w: Weight, name: str, out_dtype: torch.dtype | None):
     return km, (out_dtype or x.dtype)
 
 
-def logits_from_hidden(x: torch.Tensor, lm_head: Weight, *, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+def logits_from_hidden(x: torch.Tensor | Q8Rows, lm_head: Weight, *,
+                       out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """kappa/qwen3/transformer.py:55-59: ``einsum("btd,vd->btv")`` -> ``[B, T, vocab]``.
 
     kappa's result dtype is x's (bf16); ``out_dtype=torch.float32`` keeps
-    the fp32 sums instead.
+    the fp32 sums instead.  ``x`` may be 8-bit rows (``rms_norm_q8`` as the
+    final norm); their logits are bf16 by default as well.
     """
+    if isinstance(x, Q8Rows):
+        km, dt = _head(x, lm_head, "lm_head", out_dtype or torch.bfloat16)
+        return _dense.linear_q8(x, km, out_dtype=dt)
     km, dt = _head(x, lm_head, "lm_head", out_dtype)
     V, D = (int(s) for s in km.shape)
     _dense.check_x(x, D)

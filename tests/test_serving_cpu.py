@@ -47,3 +47,37 @@ def test_add_rms_norm_refuses(kw, code, text):
 
 def test_add_rms_norm_of_no_rows_is_nothing():
     assert _norm(T=0, x=None, residual=None, scale=None, h=None, q=None, qs=None) == L.KW8_OK
+
+
+def _linear(q=P, qs=P + (1 << 16), T=4, K=64, N=32, w=None, dt=L.DT_BF16, out=P + (1 << 18)):
+    w = w or L.KW8Weight(P + (1 << 17), P + (1 << 19), L.DT_F32, 1, L.LAYOUT_KMAJOR, 0)
+    return L.load().kw8_linear_q8(q, qs, T, K, N, w, dt, out, None)
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(q=None), L.KW8_ERR_INVALID_ARG, "null"),
+    (dict(qs=None), L.KW8_ERR_INVALID_ARG, "null"),
+    (dict(out=None), L.KW8_ERR_INVALID_ARG, "null"),
+    (dict(T=-1), L.KW8_ERR_INVALID_ARG, "bad shape"),
+    (dict(K=0), L.KW8_ERR_INVALID_ARG, "bad shape"),
+    (dict(N=0), L.KW8_ERR_INVALID_ARG, "bad shape"),
+    (dict(K=72), L.KW8_ERR_UNSUPPORTED, "multiple of 16"),
+    (dict(K=131072), L.KW8_ERR_UNSUPPORTED, "131056"),
+    (dict(T=1 << 31), L.KW8_ERR_UNSUPPORTED, "range"),
+    (dict(N=1 << 31), L.KW8_ERR_UNSUPPORTED, "range"),
+    (dict(dt=4), L.KW8_ERR_INVALID_ARG, "out dtype"),
+    (dict(q=P + 8), L.KW8_ERR_UNSUPPORTED, "aligned"),
+    (dict(out=P + (1 << 18) + 1), L.KW8_ERR_UNSUPPORTED, "aligned"),
+    (dict(out=P + (1 << 18) + 2, dt=L.DT_F32), L.KW8_ERR_UNSUPPORTED, "aligned"),
+    (dict(w=L.KW8Weight(None, P, L.DT_F32, 1, 0, 0)), L.KW8_ERR_INVALID_ARG, "null"),
+    (dict(w=L.KW8Weight(P, P, 9, 1, 0, 0)), L.KW8_ERR_INVALID_ARG, "scale dtype"),
+    (dict(w=L.KW8Weight(P, P, L.DT_F32, 1, 7, 0)), L.KW8_ERR_INVALID_ARG, "layout"),
+    (dict(w=L.KW8Weight(P + 4, P, L.DT_F32, 1, 0, 0)), L.KW8_ERR_UNSUPPORTED, "aligned"),
+])
+def test_linear_q8_refuses(kw, code, text):
+    assert _linear(**kw) == code
+    assert text in L.last_error()
+
+
+def test_linear_q8_of_no_rows_is_nothing():
+    assert _linear(T=0, q=None, qs=None, out=None) == L.KW8_OK
