@@ -244,6 +244,42 @@ int kw8_add_rms_norm(const void* x, const void* residual, int64_t T, int64_t D, 
 int kw8_dequantize_rows(const int8_t* q, const float* scale, int64_t T, int64_t D, int32_t out_dtype,
                         void* out, kw8_stream_t stream);
 
+/* ---------------------------------------------------------- sampling -- */
+
+/* The settings of kw8_sample: per row where a pointer is given (device,
+ * [B]), else the one value.                                                 */
+typedef struct kw8_sampling {
+  const float* temperatures; /* [B] or NULL                                  */
+  const int32_t* top_ks;     /* [B] or NULL                                  */
+  const float* top_ps;       /* [B] or NULL                                  */
+  const float* min_ps;       /* [B] or NULL                                  */
+  float temperature;         /* not above 0: the most likely token           */
+  int32_t top_k;             /* below 1 or above V: every token              */
+  float top_p;               /* 1 or more: every token                       */
+  float min_p;               /* 0 or less: every token                       */
+} kw8_sampling;
+
+/* One token per row of logits, from given random numbers (kappa's sampling,
+ * kappa/gemma3/sampling.py, draws its own).  Per row x, m = max x, a NaN logit
+ * counting as -inf:
+ *   w_i = floor(2^44 * exp((x_i - m) / temperature)), exp in 64 bits;
+ *   the tokens ordered by x descending, ties by index ascending;
+ *   kept: the first top_k; of these the shortest prefix whose sum of w is at
+ *   least top_p times the sum over those top_k; of these the ones with
+ *   w >= min_p * 2^44; always the first token;
+ *   token = the first index (in the order of the vocabulary) at which the
+ *   running sum of the kept w exceeds min(floor(u * sum), sum - 1), u taken
+ *   into [0, 1]; logprob = ln(w[token] / sum).
+ * temperature not above 0, top_p not above 0, min_p above 1, or a NaN in one
+ * of them: the first token of the order, logprob 0.  A row without a logit
+ * above -inf: token -1, logprob -inf.
+ *   logits: [B][V] in logits_dtype (f32 or bf16), rows row_stride elements
+ *   apart, V <= 393216; u [B] fp32; token_out [B]; logprob_out [B] or NULL.
+ * Sums are whole numbers: equal inputs give equal tokens on every call.      */
+int kw8_sample(const void* logits, int32_t logits_dtype, int64_t B, int64_t V, int64_t row_stride,
+               const float* u, const kw8_sampling* settings, int32_t* token_out, float* logprob_out,
+               kw8_stream_t stream);
+
 /* The norms around a decoder block's FFN.  pre_scale [D] (required) is the
  * pre-FFN RMSNorm; post_scale [D] (or NULL: none, as in Qwen3) the post-FFN
  * RMSNorm; both in scale_dtype, of one kind.                                */

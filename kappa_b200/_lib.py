@@ -87,6 +87,21 @@ class KW8BlockNorms(ctypes.Structure):
     ]
 
 
+class KW8Sampling(ctypes.Structure):
+    """``kw8_sampling`` (include/kappa_w8.h): one value each, or one per row."""
+
+    _fields_ = [
+        ("temperatures", ctypes.c_void_p),
+        ("top_ks", ctypes.c_void_p),
+        ("top_ps", ctypes.c_void_p),
+        ("min_ps", ctypes.c_void_p),
+        ("temperature", ctypes.c_float),
+        ("top_k", ctypes.c_int32),
+        ("top_p", ctypes.c_float),
+        ("min_p", ctypes.c_float),
+    ]
+
+
 class KW8EpPeers(ctypes.Structure):
     """``kw8_ep_peers`` (include/kappa_w8.h): an expert-parallel group seen from one rank."""
 
@@ -150,6 +165,10 @@ SIGNATURES: dict[str, tuple] = {
         [_vp, _vp, _i64, _i64, _vp, _i32, _i32, ctypes.c_float, _vp, _vp, _vp, _vp, _vp],
     ),
     "kw8_dequantize_rows": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i32, _vp, _vp]),
+    "kw8_sample": (
+        ctypes.c_int,
+        [_vp, _i32, _i64, _i64, _i64, _vp, ctypes.POINTER(KW8Sampling), _vp, _vp, _vp],
+    ),
     "kw8_dense_block_workspace_size": (_sz, [_i64, _i64, _i64]),
     "kw8_dense_block": (
         ctypes.c_int,

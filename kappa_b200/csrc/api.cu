@@ -9,6 +9,7 @@
 #include "moe.cuh"
 #include "norm.cuh"
 #include "quant.cuh"
+#include "sample.cuh"
 
 namespace kw8 {
 const char* last_error();
@@ -1004,6 +1005,46 @@ int kw8_add_rms_norm(const void* x, const void* residual, int64_t T, int64_t D, 
   KW8_API_BEGIN
   return launch_add_rms_norm(x, residual, T, D, scale, scale_dtype, kind, eps, h_out, y_out, q_out, q_scale_out,
                              stream);
+}
+
+int kw8_sample(const void* logits, int32_t logits_dtype, int64_t B, int64_t V, int64_t row_stride, const float* u,
+               const kw8_sampling* s, int32_t* token_out, float* logprob_out, kw8_stream_t stream) {
+  KW8_API_BEGIN
+  KW8_REQUIRE(B >= 0 && V > 0, KW8_ERR_INVALID_ARG, "bad shape (B=%lld V=%lld)", (long long)B, (long long)V);
+  KW8_REQUIRE(logits_dtype == KW8_DT_F32 || logits_dtype == KW8_DT_BF16, KW8_ERR_INVALID_ARG,
+              "logits must be f32 or bf16");
+  KW8_REQUIRE(V <= kSampleMaxV, KW8_ERR_UNSUPPORTED, "V=%lld is above %lld", (long long)V, (long long)kSampleMaxV);
+  KW8_REQUIRE(B < (1ll << 28), KW8_ERR_UNSUPPORTED, "too many rows");
+  KW8_REQUIRE(row_stride >= 0 && row_stride < (1ll << 40), KW8_ERR_INVALID_ARG, "bad row stride %lld",
+              (long long)row_stride);
+  KW8_REQUIRE(s != nullptr, KW8_ERR_INVALID_ARG, "null settings");
+  KW8_REQUIRE(s->temperatures || s->temperature == s->temperature, KW8_ERR_INVALID_ARG, "temperature is NaN");
+  KW8_REQUIRE(s->top_ps || s->top_p == s->top_p, KW8_ERR_INVALID_ARG, "top_p is NaN");
+  KW8_REQUIRE(s->min_ps || s->min_p == s->min_p, KW8_ERR_INVALID_ARG, "min_p is NaN");
+  if (B == 0) return KW8_OK;
+  KW8_REQUIRE(logits && u && token_out, KW8_ERR_INVALID_ARG, "null logits/u/token_out");
+  KW8_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (logits_dtype == KW8_DT_F32 ? 3 : 1)) == 0 &&
+                  ((reinterpret_cast<uintptr_t>(u) | reinterpret_cast<uintptr_t>(token_out) |
+                    reinterpret_cast<uintptr_t>(logprob_out) | reinterpret_cast<uintptr_t>(s->temperatures) |
+                    reinterpret_cast<uintptr_t>(s->top_ks) | reinterpret_cast<uintptr_t>(s->top_ps) |
+                    reinterpret_cast<uintptr_t>(s->min_ps)) & 3) == 0,
+              KW8_ERR_UNSUPPORTED, "pointers must be aligned to their type");
+  SampleArgs a{};
+  a.logits = logits;
+  a.ld = row_stride;
+  a.V = static_cast<int>(V);
+  a.u = u;
+  a.temperature = s->temperatures;
+  a.top_k = s->top_ks;
+  a.top_p = s->top_ps;
+  a.min_p = s->min_ps;
+  a.temperature0 = s->temperature;
+  a.top_k0 = s->top_k;
+  a.top_p0 = s->top_p;
+  a.min_p0 = s->min_p;
+  a.token = token_out;
+  a.logprob = logprob_out;
+  return launch_sample(a, B, logits_dtype, stream);
 }
 
 size_t kw8_dense_block_workspace_size(int64_t T, int64_t D, int64_t H) {

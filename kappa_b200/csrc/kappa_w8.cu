@@ -10,6 +10,7 @@
 #include "gemm_q8.cu"
 #include "moe.cu"
 #include "norm.cu"
+#include "sample.cu"
 #include "api.cu"
 #include "noalloc.cu"
 #include "ep.cu"

@@ -81,3 +81,46 @@ def test_linear_q8_refuses(kw, code, text):
 
 def test_linear_q8_of_no_rows_is_nothing():
     assert _linear(T=0, q=None, qs=None, out=None) == L.KW8_OK
+
+
+def _sample(logits=P, dt=L.DT_F32, B=4, V=100, ld=100, u=P + (1 << 16), s=0, token=P + (1 << 17), logprob=P + (1 << 18),
+            **kw):
+    import ctypes
+
+    s = L.KW8Sampling(None, None, None, None, kw.get("temperature", 1.0), 0, kw.get("top_p", 1.0), kw.get("min_p", 0.0)) \
+        if s == 0 else s
+    if s is not None and "temperatures" in kw:
+        s.temperatures = kw["temperatures"]
+    return L.load().kw8_sample(logits, dt, B, V, ld, u, None if s is None else ctypes.byref(s), token, logprob, None)
+
+
+NAN = float("nan")
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(logits=None), L.KW8_ERR_INVALID_ARG, "null"),
+    (dict(u=None), L.KW8_ERR_INVALID_ARG, "null"),
+    (dict(token=None), L.KW8_ERR_INVALID_ARG, "null"),
+    (dict(s=None), L.KW8_ERR_INVALID_ARG, "settings"),
+    (dict(dt=2), L.KW8_ERR_INVALID_ARG, "f32 or bf16"),
+    (dict(V=0), L.KW8_ERR_INVALID_ARG, "bad shape"),
+    (dict(B=-1), L.KW8_ERR_INVALID_ARG, "bad shape"),
+    (dict(V=393217, ld=393217), L.KW8_ERR_UNSUPPORTED, "393216"),
+    (dict(B=1 << 28), L.KW8_ERR_UNSUPPORTED, "too many"),
+    (dict(ld=-1), L.KW8_ERR_INVALID_ARG, "stride"),
+    (dict(ld=1 << 41), L.KW8_ERR_INVALID_ARG, "stride"),
+    (dict(temperature=NAN), L.KW8_ERR_INVALID_ARG, "temperature"),
+    (dict(top_p=NAN), L.KW8_ERR_INVALID_ARG, "top_p"),
+    (dict(min_p=NAN), L.KW8_ERR_INVALID_ARG, "min_p"),
+    (dict(logits=P + 2), L.KW8_ERR_UNSUPPORTED, "aligned"),
+    (dict(logits=P + 1, dt=L.DT_BF16), L.KW8_ERR_UNSUPPORTED, "aligned"),
+    (dict(token=P + 2), L.KW8_ERR_UNSUPPORTED, "aligned"),
+    (dict(temperatures=P + 1), L.KW8_ERR_UNSUPPORTED, "aligned"),
+])
+def test_sample_refuses(kw, code, text):
+    assert _sample(**kw) == code
+    assert text in L.last_error()
+
+
+def test_sample_of_no_rows_is_nothing():
+    assert _sample(B=0, logits=None, u=None, token=None) == L.KW8_OK
