@@ -14,11 +14,14 @@
 // most likely one has weight 0.
 //
 // A cluster of up to eight CTAs takes a row; each holds its slice in shared
-// memory, so the logits are read once.  All filters cut the same order, so each
-// is found as a cut (key, ties): first by a histogram of kBins bins linear in
-// (m - x) / temperature, then, inside the bin that holds the cut, by histograms
-// over the ordered bit patterns until one value is left, whose ties are kept by
-// index.  CTAs add their histograms through distributed shared memory.
+// memory, so the logits are read once.  Every filter cuts the same order, so a
+// histogram of kBins bins linear in (m - x) / temperature (a monotone function)
+// finds the bin of each cut.  Then, with M the tokens down to that bin:
+//   M <= kList: one CTA collects, sorts and finishes them (the usual settings);
+//   else (flat rows, many ties, a wide nucleus): the cut is narrowed inside its
+//   bin by histograms over the ordered bit patterns until one value is left,
+//   whose ties are kept by index, and every CTA draws from its slice.
+// CTAs add their histograms through distributed shared memory.
 #include "sample.cuh"
 
 #include <cmath>
@@ -27,11 +30,14 @@ namespace kw8 {
 
 namespace {
 
-constexpr int kSampThreads = 512;
-constexpr int kSampWarps = kSampThreads / 32;
 constexpr int kBins = 1024;
-constexpr float kBinsPerUnit = 32.f;  // bins per e-fold of the weight: the last one holds weights of 0
+constexpr float kBinSpan = 32.f;  // e-folds of the weight over all bins: the last one holds weights of 0
+constexpr int kList = 1024;       // tokens that one CTA sorts
+constexpr int kRanked = 256;      // up to here by counting, above by a sorting network
+constexpr int kMaxRanks = 16;
+constexpr int kMaxSmem = 232448;
 constexpr double kOne = 17592186044416.0;  // 2^44
+constexpr int kExpSteps = 32;         // table steps per octave of the exp (weight())
 
 using u64 = unsigned long long;
 
@@ -45,12 +51,37 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 }
 
 // NaN -> -inf, -0 -> +0.
-__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x + 0.0f; }
+__device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY) + 0.0f; }
 
 __device__ __forceinline__ float elem(const float* s, int i) { return s[i]; }
 __device__ __forceinline__ float elem(const __nv_bfloat16* s, int i) { return __bfloat162float(s[i]); }
 __device__ __forceinline__ void put(float* s, int i, float x) { s[i] = x; }
 __device__ __forceinline__ void put(__nv_bfloat16* s, int i, float x) { s[i] = __float2bfloat16_rn(x); }
+
+// The 16 / sizeof(E) values of a vector, cleaned, and back.
+__device__ __forceinline__ void unpack(const uint4& v, float (&f)[4]) {
+  f[0] = clean(__uint_as_float(v.x));
+  f[1] = clean(__uint_as_float(v.y));
+  f[2] = clean(__uint_as_float(v.z));
+  f[3] = clean(__uint_as_float(v.w));
+}
+__device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = clean(__uint_as_float(w[i] << 16));
+    f[2 * i + 1] = clean(__uint_as_float(w[i] & 0xFFFF0000u));
+  }
+}
+__device__ __forceinline__ uint4 pack(const float (&f)[4]) {
+  return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+__device__ __forceinline__ uint4 pack(const float (&f)[8]) {  // the values are bf16 numbers: the upper halves
+  return make_uint4(__byte_perm(__float_as_uint(f[0]), __float_as_uint(f[1]), 0x7632),
+                    __byte_perm(__float_as_uint(f[2]), __float_as_uint(f[3]), 0x7632),
+                    __byte_perm(__float_as_uint(f[4]), __float_as_uint(f[5]), 0x7632),
+                    __byte_perm(__float_as_uint(f[6]), __float_as_uint(f[7]), 0x7632));
+}
 
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
   uint32_t v;
@@ -62,368 +93,747 @@ __device__ __forceinline__ u64 ld_cluster_u64(uint32_t addr) {
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void st_cluster_u64(uint32_t addr, u64 v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
 
 // Shared state of a CTA besides its slice.
-struct SampShared {
-  u64 mass[kBins], mass_sum[kBins];
-  uint32_t count[kBins], count_sum[kBins];
-  u64 warp_a[kSampWarps];
-  u64 pub[2];    // this CTA's value of a cluster-wide reduction (two: alternate)
-  u64 cut[2];    // sum before the cut's bin
+struct alignas(16) SampShared {
+  // This CTA's histogram: a weight (45 bits) is added in pieces of 16, 16 and
+  // 13 bits, each a 32-bit atomic (a CTA holds under 2^16 logits, so none
+  // overflows); 64-bit atomics on shared memory are compare-and-swap loops.
+  // The list of candidates takes the same memory.
+  union {
+    uint32_t mass[3][kBins];
+    u64 list[kList];
+  };
+  uint32_t count[kBins];
+  // The cluster's histogram; the collected list and its sort take the same memory.
+  union {
+    struct {
+      u64 mass_sum[kBins];
+      uint32_t count_sum[kBins];
+    };
+    u64 gathered[kList];
+  };
+  double exp_table[kExpSteps * 16];  // 2^(-i / kExpSteps), sixteen copies side by side
+  u64 warp_a[32];
+  u64 pub[2][kMaxRanks][3];  // every CTA's values of a cluster-wide reduction (alternating)
+  u64 cut_before;            // sum in front of the cut's bin
   uint32_t cut_bin, cut_count;
+  uint32_t listed;              // tokens of this CTA down to the cut (entries of `list` while they fit)
+  uint32_t lists[kMaxRanks];    // every CTA's
 };
 
-template <class Op>
-__device__ __forceinline__ u64 block_reduce(u64 v, SampShared& sh, Op op) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh.warp_a[threadIdx.x >> 5] = v;
-  __syncthreads();
-  u64 r = sh.warp_a[0];
-  for (int i = 1; i < kSampWarps; ++i) r = op(r, sh.warp_a[i]);
-  return r;
-}
+template <int kThreads>
+struct Row {
+  static constexpr int kWarps = kThreads / 32;
+  SampShared& sh;
+  const int ranks, rank;
+  int turn = 0;
 
-// Over all CTAs of the cluster; the same value in every thread.  `turn`
-// alternates, so a value may be published while the last one is still read.
-template <class Op>
-__device__ __forceinline__ u64 cluster_reduce(u64 v, SampShared& sh, int ranks, int& turn, Op op) {
-  v = block_reduce(v, sh, op);
-  if (ranks == 1) return v;
-  turn ^= 1;
-  if (threadIdx.x == 0) sh.pub[turn] = v;
-  cluster_sync_all();
-  const uint32_t a = smem_u32(&sh.pub[turn]);
-  u64 r = ld_cluster_u64(mapa_shared(a, 0));
-  for (int i = 1; i < ranks; ++i) r = op(r, ld_cluster_u64(mapa_shared(a, static_cast<uint32_t>(i))));
-  return r;
-}
+  __device__ Row(SampShared& s, int n, int r) : sh(s), ranks(n), rank(r) {}
 
-// Exclusive prefix of v over the cluster's threads, CTA by CTA; `total` is the sum.
-__device__ __forceinline__ u64 cluster_prefix(u64 v, SampShared& sh, int ranks, int rank, int& turn, u64& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  u64 inc = v;
+  __device__ __forceinline__ void sync() {
+    if (ranks > 1)
+      cluster_sync_all();
+    else
+      __syncthreads();
+  }
+
+  template <class Op>
+  __device__ __forceinline__ u64 block_reduce(u64 v, Op op) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 n = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += n;
+    for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh.warp_a[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = sh.warp_a[(threadIdx.x & 31) % kWarps];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      if (o < kWarps) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
   }
-  __syncthreads();
-  if (lane == 31) sh.warp_a[warp] = inc;
-  __syncthreads();
-  u64 base = 0, all = 0;
-  for (int i = 0; i < kSampWarps; ++i) {
-    if (i < warp) base += sh.warp_a[i];
-    all += sh.warp_a[i];
-  }
-  total = all;
-  if (ranks > 1) {
+
+  // Stores this CTA's values into every CTA's slot for it (thread r into CTA
+  // r), and waits for all of them.  The slots alternate, so the last ones may
+  // still be read meanwhile.
+  __device__ __forceinline__ void publish(u64 a, u64 b, u64 c) {
     turn ^= 1;
-    if (threadIdx.x == 0) sh.pub[turn] = all;
+    if (static_cast<int>(threadIdx.x) < ranks) {
+      const uint32_t at = mapa_shared(smem_u32(sh.pub[turn][rank]), threadIdx.x);
+      st_cluster_u64(at, a);
+      st_cluster_u64(at + 8, b);
+      st_cluster_u64(at + 16, c);
+    }
     cluster_sync_all();
-    const uint32_t a = smem_u32(&sh.pub[turn]);
-    total = 0;
+  }
+
+  // Over all CTAs of the cluster; the same value in every thread.
+  template <class Op>
+  __device__ __forceinline__ u64 reduce(u64 v, Op op) {
+    v = block_reduce(v, op);
+    if (ranks == 1) return v;
+    publish(v, 0, 0);
+    u64 r = sh.pub[turn][0][0];
+    for (int i = 1; i < ranks; ++i) r = op(r, sh.pub[turn][i][0]);
+    return r;
+  }
+
+  // The same for a least value, a largest one and a sum at once.
+  __device__ __forceinline__ void reduce3(u64& lo, u64& hi, u64& sum) {
+    const auto mn = [](u64 a, u64 b) { return a < b ? a : b; };
+    const auto mx = [](u64 a, u64 b) { return a > b ? a : b; };
+    lo = block_reduce(lo, mn);
+    hi = block_reduce(hi, mx);
+    sum = block_reduce(sum, [](u64 a, u64 b) { return a + b; });
+    if (ranks == 1) return;
+    publish(lo, hi, sum);
+    sum = 0;
     for (int i = 0; i < ranks; ++i) {
-      const u64 c = ld_cluster_u64(mapa_shared(a, static_cast<uint32_t>(i)));
-      if (i < rank) base += c;
-      total += c;
+      lo = mn(lo, sh.pub[turn][i][0]);
+      hi = mx(hi, sh.pub[turn][i][1]);
+      sum += sh.pub[turn][i][2];
     }
   }
-  return base + inc - v;
-}
 
-__device__ __forceinline__ void clear_hist(SampShared& sh) {
-  __syncthreads();
-  for (int b = threadIdx.x; b < kBins; b += kSampThreads) {
-    sh.mass[b] = 0;
-    sh.count[b] = 0;
-  }
-  __syncthreads();
-}
-
-// Adds the CTAs' histograms: every CTA gets every bin.
-__device__ __forceinline__ void sum_hist(SampShared& sh, int ranks) {
-  if (ranks == 1) {
-    __syncthreads();
-    for (int b = threadIdx.x; b < kBins; b += kSampThreads) {
-      sh.mass_sum[b] = sh.mass[b];
-      sh.count_sum[b] = sh.count[b];
+  // Exclusive prefix of v over this CTA's threads; `all` is their sum.
+  __device__ __forceinline__ u64 block_prefix(u64 v, u64& all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    u64 inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 n = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += n;
     }
     __syncthreads();
-    return;
-  }
-  cluster_sync_all();
-  for (int b = threadIdx.x; b < kBins; b += kSampThreads) {
-    u64 m = 0;
-    uint32_t c = 0;
-    for (int i = 0; i < ranks; ++i) {
-      m += ld_cluster_u64(mapa_shared(smem_u32(&sh.mass[b]), static_cast<uint32_t>(i)));
-      c += ld_cluster_u32(mapa_shared(smem_u32(&sh.count[b]), static_cast<uint32_t>(i)));
+    if (lane == 31) sh.warp_a[warp] = inc;
+    __syncthreads();
+    u64 base = 0;
+    all = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      const u64 c = sh.warp_a[i];
+      if (i < warp) base += c;
+      all += c;
     }
-    sh.mass_sum[b] = m;
-    sh.count_sum[b] = c;
+    return base + inc - v;
   }
-  cluster_sync_all();  // the histograms may be cleared again
-}
 
-struct Target {
-  bool by_mass;
-  u64 k;       // by count: the k-th
-  double thr;  // by mass: the first whose running sum is not below thr
+  // The same over the cluster's threads, CTA by CTA.
+  __device__ __forceinline__ u64 prefix(u64 v, u64& total) {
+    u64 all;
+    u64 at = block_prefix(v, all);
+    total = all;
+    if (ranks > 1) {
+      publish(all, 0, 0);
+      total = 0;
+      for (int i = 0; i < ranks; ++i) {
+        const u64 c = sh.pub[turn][i][0];
+        if (i < rank) at += c;
+        total += c;
+      }
+    }
+    return at;
+  }
+
+  __device__ __forceinline__ void clear(bool mass) {
+    __syncthreads();
+    for (int b = threadIdx.x; b < kBins; b += kThreads) {
+      if (mass)
+        sh.mass[0][b] = sh.mass[1][b] = sh.mass[2][b] = 0;
+      sh.count[b] = 0;
+    }
+    __syncthreads();
+  }
+
+  __device__ __forceinline__ void add_mass(int b, u64 w) {
+    if (w == 0) return;
+    atomicAdd(&sh.mass[0][b], static_cast<uint32_t>(w) & 0xFFFFu);
+    atomicAdd(&sh.mass[1][b], static_cast<uint32_t>(w >> 16) & 0xFFFFu);
+    atomicAdd(&sh.mass[2][b], static_cast<uint32_t>(w >> 32));
+  }
+
+  // Adds the CTAs' histograms: each sums its share of the bins, some threads
+  // to a bin, and stores it into every CTA's copy.
+  __device__ __forceinline__ void sum(bool count, bool mass) {
+    sync();
+    const int share = (kBins + ranks - 1) / ranks;
+    const int group = ranks >= 4 && kThreads >= 4 * share ? 4 : ranks >= 2 && kThreads >= 2 * share ? 2 : 1;
+    const int part = static_cast<int>(threadIdx.x) % group;
+    const int b0 = rank * share, b1 = min(kBins, b0 + share);
+    // Whole warps go around together: the shuffles need them.
+    for (int base = b0; base < b1; base += kThreads / group) {
+      const int b = base + static_cast<int>(threadIdx.x) / group;
+      const bool valid = b < b1;
+      u64 m = 0;
+      uint32_t c = 0;
+      if (valid)
+        for (int i = part; i < ranks; i += group) {
+          const uint32_t r = static_cast<uint32_t>(i);
+          if (count) c += ld_cluster_u32(mapa_shared(smem_u32(&sh.count[b]), r));
+          if (mass)
+            m += ld_cluster_u32(mapa_shared(smem_u32(&sh.mass[0][b]), r)) +
+                 (static_cast<u64>(ld_cluster_u32(mapa_shared(smem_u32(&sh.mass[1][b]), r))) << 16) +
+                 (static_cast<u64>(ld_cluster_u32(mapa_shared(smem_u32(&sh.mass[2][b]), r))) << 32);
+        }
+      for (int o = 1; o < group; o <<= 1) {
+        c += __shfl_xor_sync(0xffffffffu, c, o);
+        m += __shfl_xor_sync(0xffffffffu, m, o);
+      }
+      if (valid)
+        for (int i = part; i < ranks; i += group) {
+          const uint32_t r = static_cast<uint32_t>(i);
+          st_cluster_u32(mapa_shared(smem_u32(&sh.count_sum[b]), r), c);
+          if (mass) st_cluster_u64(mapa_shared(smem_u32(&sh.mass_sum[b]), r), m);
+        }
+    }
+    sync();  // the sums are complete, and the histograms may be cleared again
+  }
+
+  // Finds the bin in which the running sum (of the counts: up to k; of the
+  // masses: up to thr), `before` in front of bin 0, reaches its goal, and leaves
+  // it in sh: the bin, its count and the sum in front of it.
+  __device__ __forceinline__ void find_cut(bool by_mass, u64 k, double thr, u64 before) {
+    constexpr int kPer = kBins / kThreads;
+    u64 v[kPer], s = 0, all;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int b = threadIdx.x * kPer + j;
+      v[j] = by_mass ? sh.mass_sum[b] : sh.count_sum[b];
+      s += v[j];
+    }
+    u64 at = before + block_prefix(s, all);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const u64 next = at + v[j];
+      const bool here = by_mass ? (static_cast<double>(at) < thr && !(static_cast<double>(next) < thr))
+                                : (at < k && next >= k);
+      if (here) {
+        sh.cut_bin = static_cast<uint32_t>(threadIdx.x * kPer + j);
+        sh.cut_count = sh.count_sum[threadIdx.x * kPer + j];
+        sh.cut_before = at;
+      }
+      at = next;
+    }
+    __syncthreads();
+  }
+
+  // a[0 .. size) into descending order; size a power of two.
+  __device__ __forceinline__ void sort(u64* a, int size) {
+    for (int len = 2; len <= size; len <<= 1)
+      for (int step = len >> 1; step > 0; step >>= 1) {
+        for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+          const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
+          const u64 p = a[lo], q = a[hi];
+          if ((p < q) == ((lo & len) == 0)) {
+            a[lo] = q;
+            a[hi] = p;
+          }
+        }
+        __syncthreads();
+      }
+  }
 };
 
-// Finds the bin in which the running sum, `before` in front of bin 0, reaches
-// the target; leaves (bin, its count, the sum in front of it) in sh.
-__device__ __forceinline__ void find_cut(SampShared& sh, const Target& t, u64 before) {
-  constexpr int kPer = kBins / kSampThreads;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  u64 v[kPer], sum = 0;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int b = threadIdx.x * kPer + j;
-    v[j] = t.by_mass ? sh.mass_sum[b] : sh.count_sum[b];
-    sum += v[j];
-  }
-  u64 inc = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 n = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += n;
-  }
-  __syncthreads();
-  if (lane == 31) sh.warp_a[warp] = inc;
-  __syncthreads();
-  u64 at = before + inc - sum;
-  for (int i = 0; i < warp; ++i) at += sh.warp_a[i];
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const u64 next = at + v[j];
-    const bool here = t.by_mass ? (static_cast<double>(at) < t.thr && !(static_cast<double>(next) < t.thr))
-                                : (at < t.k && next >= t.k);
-    if (here) {
-      sh.cut_bin = static_cast<uint32_t>(threadIdx.x * kPer + j);
-      sh.cut_count = sh.count_sum[threadIdx.x * kPer + j];
-      sh.cut[0] = at;
-    }
-    at = next;
-  }
-  __syncthreads();
-}
+__device__ __forceinline__ u64 max64(u64 a, u64 b) { return a > b ? a : b; }
+__device__ __forceinline__ u64 min64(u64 a, u64 b) { return a < b ? a : b; }
+__device__ __forceinline__ u64 add64(u64 a, u64 b) { return a + b; }
 
-template <class E>
-__global__ void __launch_bounds__(kSampThreads)
+template <class E, int kThreads>
+__global__ void __launch_bounds__(kThreads)
     sample_kernel(const SampleArgs p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   SampShared& sh = *reinterpret_cast<SampShared*>(smem_raw);
-  E* x = reinterpret_cast<E*>(smem_raw + sizeof(SampShared));
   uint32_t ranks_u;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks_u));
-  const int ranks = static_cast<int>(ranks_u), rank = static_cast<int>(cluster_ctarank());
+  const int ranks = static_cast<int>(ranks_u), rank = ranks > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  Row<kThreads> R(sh, ranks, rank);
+  const int tid = static_cast<int>(threadIdx.x);
   const int64_t row = blockIdx.x / ranks;
   const int first = rank * p.slice;
   const int n = max(0, min(p.slice, p.V - first));
-  const E* src = static_cast<const E*>(p.logits) + row * p.ld + first;
-  int turn = 0;
-
-  // The slice, and the row's first largest logit.
-  u64 best = 0;  // (key, ~index): the largest value, of these the lowest index
-  for (int i = threadIdx.x; i < n; i += kSampThreads) {
-    const float v = clean(elem(src, i));
-    put(x, i, v);
-    best = max(best, (static_cast<u64>(order_key(v)) << 32) | (0xffffffffu - static_cast<uint32_t>(first + i)));
-  }
-  best = cluster_reduce(best, sh, ranks, turn, [](u64 a, u64 b) { return a > b ? a : b; });
-  const uint32_t top_key = static_cast<uint32_t>(best >> 32);
-  const float top = key_value(top_key);
-  const int top_index = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
+  const E* src = static_cast<const E*>(p.logits) + row * p.ld + (n > 0 ? first : 0);
 
   const float temp = p.temperature ? p.temperature[row] : p.temperature0;
   const float top_p = p.top_p ? p.top_p[row] : p.top_p0;
   const float min_p = p.min_p ? p.min_p[row] : p.min_p0;
   const int32_t k = p.top_k ? p.top_k[row] : p.top_k0;
+  for (int i = tid; i < kExpSteps * 16; i += kThreads) sh.exp_table[i] = exp2(-(i >> 4) * (1.0 / kExpSteps));
+  if (tid == 0) sh.listed = 0;
 
-  if (top == -INFINITY || !(temp > 0.f) || !(top_p > 0.f) || !(min_p <= 1.f) || k == 1) {
-    // No token at all, or the first most likely one.
-    if (rank == 0 && threadIdx.x == 0) {
-      const bool none = top == -INFINITY;
-      p.token[row] = none ? -1 : top_index;
-      if (p.logprob) p.logprob[row] = none ? -INFINITY : 0.f;
+  // The slice into shared memory, at the alignment that it has in global
+  // memory (whole vectors inside, single values at the ends), and the row's
+  // first largest logit.
+  constexpr int kVec = 16 / sizeof(E);
+  const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(E));
+  E* const aligned = reinterpret_cast<E*>(smem_raw + sizeof(SampShared));
+  E* const x = aligned + lead;
+  float best = -INFINITY;
+  int best_at = -1;  // none above -inf yet
+  {
+    const uint4* gsrc = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(src) & ~static_cast<uintptr_t>(15));
+    const int v0 = (lead + kVec - 1) / kVec, v1 = (lead + n) / kVec;
+    const int head = min(n, v0 * kVec - lead), tail = max(head, v1 * kVec - lead);
+    constexpr int kUnroll = 8;
+    for (int i = tid; i < head; i += kThreads) {  // fewer than kVec: one per thread
+      const float f = clean(elem(src, i));
+      put(x, i, f);
+      if (f > best) best = f, best_at = i;
     }
-    if (ranks > 1) cluster_sync_all();
+    for (int base = v0 + tid; base < v1; base += kUnroll * kThreads) {
+      uint4 v[kUnroll];
+#pragma unroll
+      for (int j = 0; j < kUnroll; ++j)
+        if (base + j * kThreads < v1) v[j] = __ldg(gsrc + base + j * kThreads);
+#pragma unroll
+      for (int j = 0; j < kUnroll; ++j)
+        if (base + j * kThreads < v1) {
+          float f[kVec];
+          unpack(v[j], f);
+          const int i = (base + j * kThreads) * kVec;
+#pragma unroll
+          for (int e = 0; e < kVec; ++e)
+            if (f[e] > best) best = f[e], best_at = i + e - lead;
+          *reinterpret_cast<uint4*>(aligned + i) = pack(f);
+        }
+    }
+    for (int i = tail + tid; i < n; i += kThreads) {
+      const float f = clean(elem(src, i));
+      put(x, i, f);
+      if (f > best) best = f, best_at = i;
+    }
+  }
+  // (key, ~index): the largest value, of equals the lowest index.
+  const u64 best_all = R.reduce(
+      best_at < 0 ? 0 : (static_cast<u64>(order_key(best)) << 32) | (0xffffffffu - static_cast<uint32_t>(first + best_at)),
+      max64);
+  if (best_all == 0 || !(temp > 0.f) || !(top_p > 0.f) || !(min_p <= 1.f) || k == 1) {
+    // No token at all, or the first most likely one.
+    if (rank == 0 && tid == 0) {
+      p.token[row] = best_all == 0 ? -1 : static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(best_all));
+      if (p.logprob) p.logprob[row] = best_all == 0 ? -INFINITY : 0.f;
+    }
+    if (ranks > 1) cluster_sync_all();  // no CTA leaves while another reads its shared memory
     return;
   }
+  const float top = key_value(static_cast<uint32_t>(best_all >> 32));
 
-  const double inv_t = 1.0 / static_cast<double>(temp);
-  const float bin_scale = fminf(kBinsPerUnit / temp, 1e30f);
+  // floor(2^44 exp(-d / temperature)), d = m - v, by Tang's table-driven
+  // exponential: d in steps of ln2 / 32, 2^(-n/32) from the table, the rest (at
+  // most ln2 / 64) by its series to the 6th power (error below 4e-18), rounded
+  // down to 2^-44 in the bits.  No branches, so that several run at once; sixteen
+  // copies of the table, so that lanes do not meet in a bank.
+  const double top_d = static_cast<double>(top);
+  const double per_step = kExpSteps * 1.4426950408889634 / static_cast<double>(temp);
+  const uint32_t d_end = static_cast<uint32_t>(__double2hiint(46 * 0.6931471805599453 * static_cast<double>(temp)));
+  const double* const table = sh.exp_table + (tid & 15);
   const auto weight = [&](float v) -> u64 {
-    if (v == top) return static_cast<u64>(kOne);
-    if (v == -INFINITY || top == INFINITY) return 0;
-    return static_cast<u64>(exp((static_cast<double>(v) - static_cast<double>(top)) * inv_t) * kOne);
+    constexpr double h = -0.6931471805599453 / kExpSteps;
+    const double d = top_d - static_cast<double>(v);
+    const double z = fma(d, per_step, 6755399441055744.0);  // 1.5 * 2^52: the low word is the nearest integer
+    const double f = fma(d, per_step, 6755399441055744.0 - z);
+    const int steps = __double2loint(z);
+    double e = fma(f, h * h * h * h * h * h / 720, h * h * h * h * h / 120);
+    e = fma(e, f, h * h * h * h / 24);
+    e = fma(e, f, h * h * h / 6);
+    e = fma(e, f, h * h / 2);
+    e = fma(e, f, h);
+    e = fma(e, f, 1.0);
+    e *= table[(steps & (kExpSteps - 1)) * 16];
+    // e = (1.mantissa) 2^(exponent - 1023): 2^(44 - octaves) e rounded down is a shift.
+    const u64 bits = static_cast<u64>(__double_as_longlong(e));
+    const u64 w = ((bits & 0xFFFFFFFFFFFFFull) | 0x10000000000000ull) >>
+                  ((1031 - static_cast<int>(bits >> 52) + (steps >> 5)) & 63);
+    // From 46 octaves on, +inf and NaN (inf - inf, inf * 0) nothing is left.
+    const bool far = static_cast<uint32_t>(__double2hiint(d)) >= d_end;
+    return v == top ? 1ull << 44 : far ? 0 : w;
   };
-  // Monotone in v: a subtraction, a product and a truncation.
+  // Monotone in v: a subtraction, a product cut to [0, 1], a product rounded
+  // down (by adding 2^23).  +inf on both sides gives -inf, bin 0.
+  const float bin_top = fminf(top, 3.4028235e38f), bin_scale = fminf(1.f / (kBinSpan * temp), 1e30f);
   const auto bin_of = [&](float v) -> int {
-    const float d = v == top ? 0.f : (top - v) * bin_scale;
-    return static_cast<int>(fminf(d, static_cast<float>(kBins - 1)));
+    const float d = __saturatef((bin_top - v) * bin_scale);
+    return static_cast<int>(__float_as_uint(__fmaf_rz(d, static_cast<float>(kBins - 1), 8388608.f)) & (kBins - 1));
   };
 
-  // The cut: tokens above cut_key stay, of those at it the first cut_ties.
+  const bool use_k = k > 0 && k < p.V, use_p = top_p < 1.f, use_m = min_p > 0.f;
+  // w >= min_p 2^44 in whole numbers (the product is exact).
+  const u64 least = use_m ? static_cast<u64>(ceil(static_cast<double>(min_p) * kOne)) : 0;
+  const double u = fmin(fmax(static_cast<double>(p.u[row]), 0.0), 1.0);
+
+  // The cut of the general path: tokens above cut_key stay, of those at it the first cut_ties.
   uint32_t cut_key = 0;
   uint32_t cut_ties = 0xffffffffu, cut_all = 0xffffffffu;  // kept, and present
-  u64 ties_w = 0;
 
-  // Inside bin `bin` (count elements, `before` the sum in front of it): the cut's key, its ties and how many of them stay.
-  const auto refine = [&](const Target& t) {
-    u64 before = sh.cut[0];
-    uint32_t count = sh.cut_count;
-    const int bin = static_cast<int>(sh.cut_bin);
-    uint32_t lo = 0xffffffffu, hi = 0;
-    for (int i = threadIdx.x; i < n; i += kSampThreads) {
-      const float v = elem(x, i);
-      if (bin_of(v) == bin) {
-        const uint32_t key = order_key(v);
-        lo = min(lo, key);
-        hi = max(hi, key);
+  const auto count_all = [&] {
+#pragma unroll 8
+    for (int i = tid; i < n; i += kThreads) atomicAdd(&sh.count[bin_of(elem(x, i))], 1u);
+  };
+  if (use_k || use_p || use_m) {
+    const bool mass = use_p && !use_k;
+    // The histogram that finds the first cut: of the masses, or of the counts.
+    // When at least top_k threads hold a token, the top_k-th largest of the
+    // threads' own largest logits already bounds the cut (that many tokens are
+    // not below it), at one addition per thread instead of one per token.
+    int last = kBins - 1;  // nothing kept lies behind this bin
+    double thr = 0.0;
+    const bool by_threads = use_k && k <= kThreads * ranks / 2 && p.V >= kThreads * ranks;
+    if (use_k || use_p) {
+      R.clear(mass);
+      if (mass) {
+        u64 sum = 0;
+#pragma unroll 8
+        for (int i = tid; i < n; i += kThreads) {
+          const float v = elem(x, i);
+          const u64 w = weight(v);
+          sum += w;
+          R.add_mass(bin_of(v), w);
+        }
+        R.sum(false, true);
+        sum = R.reduce(sum, add64);
+        thr = static_cast<double>(top_p) * static_cast<double>(sum);
+      } else {
+        if (by_threads) {
+          if (best_at >= 0) atomicAdd(&sh.count[bin_of(best)], 1u);
+        } else {
+          count_all();
+        }
+        R.sum(true, false);
       }
+      // Fewer threads than top_k above -inf: no bound, every token may be kept.
+      sh.cut_bin = kBins - 1;
+      __syncthreads();
+      R.find_cut(mass, static_cast<u64>(k), thr, 0);
+      last = static_cast<int>(sh.cut_bin);
     }
-    lo = static_cast<uint32_t>(cluster_reduce(lo, sh, ranks, turn, [](u64 a, u64 b) { return a < b ? a : b; }));
-    hi = static_cast<uint32_t>(cluster_reduce(hi, sh, ranks, turn, [](u64 a, u64 b) { return a > b ? a : b; }));
-    while (lo != hi) {
-      const int bits = 32 - __clz(static_cast<int>(hi - lo));
-      const int shift = max(0, bits - 10);
-      clear_hist(sh);
-      for (int i = threadIdx.x; i < n; i += kSampThreads) {
-        const float v = elem(x, i);
-        const uint32_t key = order_key(v);
-        if (key >= lo && key <= hi) {
-          const uint32_t b = (hi - key) >> shift;
-          atomicAdd(&sh.count[b], 1u);
-          if (t.by_mass) atomicAdd(&sh.mass[b], weight(v));
+    // w >= min_p 2^44 means (m - x) / temperature <= -ln min_p; two bins cover
+    // the roundings.  (With top-k and top-p the list has to hold all top_k.)
+    if (use_m && !(use_k && use_p))
+      last = min(last, static_cast<int>(fminf(-logf(min_p) * ((kBins - 1) / kBinSpan), static_cast<float>(kBins))) + 2);
+
+    // Collect the tokens down to bin `last` as (key, ~index), as far as they fit.
+    // The bin as a bound on the logit: half a bin and two steps of the format
+    // lower, which covers the roundings (a few tokens too many do no harm).
+    const float low = bin_top - (static_cast<float>(last) + 1.5f) / static_cast<float>(kBins - 1) / bin_scale;
+    const uint32_t low_key = order_key(clean(low));
+    const float bound = low_key > 0x00800001u && last < kBins - 1 ? key_value(low_key - 2) : -INFINITY;
+    for (int base = tid; base < n; base += 8 * kThreads) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = base + j * kThreads;
+        const float v = elem(x, min(i, n - 1));
+        if (i < n && v >= bound) {
+          const uint32_t at = atomicAdd(&sh.listed, 1u);
+          if (at < kList) sh.list[at] = (static_cast<u64>(order_key(v)) << 32) | (0xffffffffu - static_cast<uint32_t>(first + i));
         }
       }
-      sum_hist(sh, ranks);
-      find_cut(sh, t, before);
-      before = sh.cut[0];
-      count = sh.cut_count;
-      const u64 b = sh.cut_bin;
-      const u64 new_hi = hi - (b << shift);
-      const u64 span = (1ull << shift) - 1;
-      lo = new_hi - lo > span ? static_cast<uint32_t>(new_hi - span) : lo;
-      hi = static_cast<uint32_t>(new_hi);
-    }
-    // One value left.
-    const u64 w = weight(key_value(lo));
-    uint32_t ties;
-    if (t.by_mass) {
-      uint32_t a = 1, b = count;  // the first always stays: `before` is below thr
-      while (a < b) {
-        const uint32_t mid = a + (b - a + 1) / 2;
-        if (static_cast<double>(before + static_cast<u64>(mid - 1) * w) < t.thr) a = mid; else b = mid - 1;
-      }
-      ties = a;
-    } else {
-      ties = static_cast<uint32_t>(t.k - before);
-    }
-    if (lo > cut_key || (lo == cut_key && ties < cut_ties)) {
-      cut_key = lo;
-      cut_ties = ties;
-      cut_all = count;
-      ties_w = w;
+      if (*static_cast<volatile uint32_t*>(&sh.listed) > kList) break;  // too many already
     }
     __syncthreads();
-  };
+    if (ranks > 1) {
+      if (tid < ranks) st_cluster_u32(mapa_shared(smem_u32(&sh.lists[rank]), static_cast<uint32_t>(tid)), sh.listed);
+      cluster_sync_all();
+    }
+    int M = 0, my_place = 0;
+    if (ranks > 1)
+      for (int r = 0; r < ranks; ++r) M += static_cast<int>(sh.lists[r]);
+    else
+      M = static_cast<int>(sh.listed);
 
-  if (k > 0 && k < p.V) {
-    clear_hist(sh);
-    for (int i = threadIdx.x; i < n; i += kSampThreads) atomicAdd(&sh.count[bin_of(elem(x, i))], 1u);
-    sum_hist(sh, ranks);
-    const Target t{false, static_cast<u64>(k), 0.0};
-    find_cut(sh, t, 0);
-    // In the last bin every weight is 0: whatever is kept of it is never drawn.
-    if (sh.cut_bin < kBins - 1) refine(t);
-    __syncthreads();
-  }
-  if (top_p < 1.f) {
-    clear_hist(sh);
-    u64 sum = 0;
-    for (int i = threadIdx.x; i < n; i += kSampThreads) {
-      const float v = elem(x, i);
-      const int b = bin_of(v);
-      if (b < kBins - 1 && order_key(v) >= cut_key) {
-        const u64 w = weight(v);
-        sum += w;
-        atomicAdd(&sh.mass[b], w);
-        atomicAdd(&sh.count[b], 1u);
+    if (M <= kList) {
+      // CTA 0 finishes.  Each CTA's list goes behind the ones before it.
+      if (ranks > 1) {
+        for (int r = 0; r < rank; ++r) my_place += static_cast<int>(sh.lists[r]);
+        for (int i = tid; i < static_cast<int>(sh.lists[rank]); i += kThreads)
+          st_cluster_u64(mapa_shared(smem_u32(&sh.gathered[my_place + i]), 0), sh.list[i]);
+        cluster_sync_all();
+        if (rank != 0) return;
+      } else {
+        for (int i = tid; i < M; i += kThreads) sh.gathered[i] = sh.list[i];
+        __syncthreads();
       }
+      const int limit = use_k ? min(M, k) : M;
+      if (M <= kRanked) {
+        // Each token's place: how many come before it.  kGroup threads per token.
+        constexpr int kGroup = kThreads / kRanked;
+        const int i = tid / kGroup, part = tid % kGroup;
+        u64* const weights = sh.list;
+        const u64 e = i < M ? sh.gathered[i] : 0;
+        int place = 0;
+        for (int j = part; j < M; j += kGroup) place += sh.gathered[j] > e;
+#pragma unroll
+        for (int o = 1; o < kGroup; o <<= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+        const bool in = i < M && place < limit;
+        const u64 w0 = in ? weight(key_value(static_cast<uint32_t>(e >> 32))) : 0;
+        if (part == 0 && i < M) weights[place] = w0;
+        __syncthreads();
+        u64 before, total;  // running sum in front of place `tid`
+        const u64 wp = tid < M ? weights[tid] : 0;
+        before = R.block_prefix(wp, total);
+        const double goal_p = mass ? thr : static_cast<double>(top_p) * static_cast<double>(total);
+        const bool keep = tid == 0 || (tid < limit && (!use_p || static_cast<double>(before) < goal_p) &&
+                                       wp >= least);
+        // The kept ones are the first places: their number, and their sum.
+        const u64 both = R.block_reduce(keep ? before + wp : 0, max64);
+        total = both;
+        const int kept = static_cast<int>(R.block_reduce(keep ? tid + 1 : 0, max64));
+        // In the order of the vocabulary: the sum of the kept ones with a lower index.
+        const u64 w = in && place < kept ? w0 : 0;
+        __syncthreads();
+        if (part == 0 && i < M) weights[i] = w;
+        __syncthreads();
+        const uint32_t id = static_cast<uint32_t>(e);  // ~index: higher means earlier
+        u64 run = 0;
+        for (int j = part; j < M; j += kGroup) run += static_cast<uint32_t>(sh.gathered[j]) > id ? weights[j] : 0;
+#pragma unroll
+        for (int o = 1; o < kGroup; o <<= 1) run += __shfl_xor_sync(0xffffffffu, run, o);
+        const u64 goal = min64(static_cast<u64>(u * static_cast<double>(total)), total - 1);
+        if (part == 0 && w != 0 && run <= goal && goal < run + w) {
+          p.token[row] = static_cast<int32_t>(0xffffffffu - id);
+          if (p.logprob) p.logprob[row] = static_cast<float>(log(static_cast<double>(w) / static_cast<double>(total)));
+        }
+        return;
+      }
+      int size = 64;
+      while (size < M) size *= 2;
+      for (int i = M + tid; i < size; i += kThreads) sh.gathered[i] = 0;
+      __syncthreads();
+      R.sort(sh.gathered, size);
+      // Thread t owns the kPer places from t * kPer on.
+      constexpr int kPer = (kList + kThreads - 1) / kThreads;
+      u64 e[kPer], w[kPer], mine = 0, total;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int i = tid * kPer + j;
+        e[j] = i < limit ? sh.gathered[i] : 0;
+        w[j] = i < limit ? weight(key_value(static_cast<uint32_t>(e[j] >> 32))) : 0;
+        mine += w[j];
+      }
+      u64 before = R.block_prefix(mine, total);
+      const double goal_p = mass ? thr : static_cast<double>(top_p) * static_cast<double>(total);
+      u64 kept = 0;
+      mine = 0;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int i = tid * kPer + j;
+        const bool keep =
+            i == 0 || (i < limit && (!use_p || static_cast<double>(before) < goal_p) && w[j] >= least);
+        before += w[j];
+        if (!keep) w[j] = 0;
+        kept += keep;
+        mine += w[j];
+      }
+      kept = R.block_reduce(kept, add64);  // the first `kept` places
+      total = R.block_reduce(mine, add64);
+      // In the order of the vocabulary: descending ~index, with the place; weights go to `list`.
+      u64* const weights = sh.list;
+      size = 64;
+      while (size < static_cast<int>(kept)) size *= 2;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int i = tid * kPer + j;
+        if (i < size) {
+          sh.gathered[i] = i < static_cast<int>(kept) ? (e[j] << 32) | static_cast<uint32_t>(i) : 0;
+          weights[i] = w[j];
+        }
+      }
+      __syncthreads();
+      R.sort(sh.gathered, size);
+      mine = 0;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int i = tid * kPer + j;
+        e[j] = i < static_cast<int>(kept) ? sh.gathered[i] : 0;
+        w[j] = i < static_cast<int>(kept) ? weights[static_cast<uint32_t>(e[j])] : 0;
+        mine += w[j];
+      }
+      u64 all;
+      u64 run = R.block_prefix(mine, all);
+      const u64 goal = min64(static_cast<u64>(u * static_cast<double>(total)), total - 1);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        if (run <= goal && goal < run + w[j]) {
+          p.token[row] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(e[j] >> 32));
+          if (p.logprob) p.logprob[row] = static_cast<float>(log(static_cast<double>(w[j]) / static_cast<double>(total)));
+        }
+        run += w[j];
+      }
+      return;
     }
-    sum = cluster_reduce(sum, sh, ranks, turn, [](u64 a, u64 b) { return a + b; });
-    if (cut_ties < cut_all) sum -= static_cast<u64>(cut_all - cut_ties) * ties_w;
-    sum_hist(sh, ranks);
-    const Target t{true, 0, static_cast<double>(top_p) * static_cast<double>(sum)};
-    find_cut(sh, t, 0);
-    refine(t);
+
+    // The general path.  Inside the bin that sh's cut is in: the cut's key, its ties and how many of them stay.
+    u64 ties_w = 0;
+    const auto refine = [&](bool by_mass, u64 goal_k, double goal_p) {
+      u64 before = sh.cut_before;
+      const int bin = static_cast<int>(sh.cut_bin);
+      u64 lo = 0xffffffffu, hi = 0, count = 0;
+      for (int i = tid; i < n; i += kThreads) {
+        const float v = elem(x, i);
+        if (bin_of(v) == bin) {
+          const uint32_t key = order_key(v);
+          lo = min64(lo, key);
+          hi = max64(hi, key);
+          ++count;
+        }
+      }
+      R.reduce3(lo, hi, count);
+      while (lo != hi) {
+        const int bits = 32 - __clz(static_cast<int>(hi - lo));
+        const int shift = max(0, bits - 10);
+        R.clear(by_mass);
+        for (int i = tid; i < n; i += kThreads) {
+          const float v = elem(x, i);
+          const uint32_t key = order_key(v);
+          if (key >= lo && key <= hi) {
+            const int b = static_cast<int>((hi - key) >> shift);
+            atomicAdd(&sh.count[b], 1u);
+            if (by_mass) R.add_mass(b, weight(v));
+          }
+        }
+        R.sum(true, by_mass);
+        R.find_cut(by_mass, goal_k, goal_p, before);
+        before = sh.cut_before;
+        count = sh.cut_count;
+        hi -= static_cast<u64>(sh.cut_bin) << shift;
+        const u64 span = (1ull << shift) - 1;
+        if (hi - lo > span) lo = hi - span;
+      }
+      // One value left.
+      const uint32_t key = static_cast<uint32_t>(lo);
+      const u64 w = weight(key_value(key));
+      uint32_t ties;
+      if (by_mass) {
+        uint32_t a = 1, b = static_cast<uint32_t>(count);  // the first always stays: `before` is below the goal
+        while (a < b) {
+          const uint32_t mid = a + (b - a + 1) / 2;
+          if (static_cast<double>(before + static_cast<u64>(mid - 1) * w) < goal_p) a = mid; else b = mid - 1;
+        }
+        ties = a;
+      } else {
+        ties = static_cast<uint32_t>(goal_k - before);
+      }
+      if (key > cut_key || (key == cut_key && ties < cut_ties)) {
+        cut_key = key;
+        cut_ties = ties;
+        cut_all = static_cast<uint32_t>(count);
+        ties_w = w;
+      }
+      __syncthreads();
+    };
+
+    if (by_threads) {
+      R.clear(false);
+      count_all();
+      R.sum(true, false);
+      R.find_cut(false, static_cast<u64>(k), 0.0, 0);
+    }
+    // In the last bin every weight is 0: whatever is kept of it is never drawn.
+    if ((use_k || use_p) && sh.cut_bin < kBins - 1) refine(mass, static_cast<u64>(k), thr);
+    if (use_k && use_p) {
+      R.clear(true);
+      u64 s = 0;
+      for (int i = tid; i < n; i += kThreads) {
+        const float v = elem(x, i);
+        if (order_key(v) >= cut_key) {
+          const u64 w = weight(v);
+          s += w;
+          R.add_mass(bin_of(v), w);
+        }
+      }
+      s = R.reduce(s, add64);
+      if (cut_ties < cut_all) s -= static_cast<u64>(cut_all - cut_ties) * ties_w;
+      R.sum(false, true);
+      const double goal = static_cast<double>(top_p) * static_cast<double>(s);
+      R.find_cut(true, 0, goal, 0);
+      refine(true, 0, goal);
+    }
   }
 
   // The draw.  Each thread owns a run of neighbouring tokens.
-  const double least = static_cast<double>(min_p) * kOne;
-  const int run = ((n + kSampThreads - 1) / kSampThreads) | 1;  // odd: no bank conflicts
-  const int i0 = min(n, static_cast<int>(threadIdx.x) * run), i1 = min(n, i0 + run);
+  const int run = ((n + kThreads - 1) / kThreads) | 1;  // odd: no bank conflicts
+  const int i0 = min(n, tid * run), i1 = min(n, i0 + run);
   u64 rank_of_tie = 0;
   if (cut_ties < cut_all) {
-    u64 mine = 0, all;
-    for (int i = i0; i < i1; ++i) mine += order_key(elem(x, i)) == cut_key;
-    rank_of_tie = cluster_prefix(mine, sh, ranks, rank, turn, all);
+    u64 ties = 0, all;
+    for (int i = i0; i < i1; ++i) ties += order_key(elem(x, i)) == cut_key;
+    rank_of_tie = R.prefix(ties, all);
   }
-  const auto kept = [&](float v, u64& tie) -> u64 {
-    const uint32_t key = order_key(v);
-    if (key < cut_key) return 0;
-    if (key == cut_key && tie++ >= cut_ties) return 0;
-    const u64 w = weight(v);
-    return static_cast<double>(w) >= least ? w : 0;
-  };
-  u64 mine = 0, tie = rank_of_tie, total;
-  for (int i = i0; i < i1; ++i) mine += kept(elem(x, i), tie);
-  u64 at = cluster_prefix(mine, sh, ranks, rank, turn, total);
-  const double u = fmin(fmax(static_cast<double>(p.u[row]), 0.0), 1.0);
-  const u64 goal = min(static_cast<u64>(u * static_cast<double>(total)), total - 1);
-  if (at <= goal && goal < at + mine) {
-    tie = rank_of_tie;
+  u64 mine = 0, total;
+  if (cut_key == 0 && !use_m) {
+#pragma unroll 8
+    for (int i = i0; i < i1; ++i) mine += weight(elem(x, i));
+  } else {
+    u64 tie = rank_of_tie;
     for (int i = i0; i < i1; ++i) {
-      const u64 w = kept(elem(x, i), tie);
-      if (goal < at + w) {
-        p.token[row] = first + i;
-        if (p.logprob) p.logprob[row] = static_cast<float>(log(static_cast<double>(w) / static_cast<double>(total)));
+      const float v = elem(x, i);
+      const uint32_t key = order_key(v);
+      if (key > cut_key || (key == cut_key && tie++ < cut_ties)) {
+        const u64 w = weight(v);
+        if (w >= least) mine += w;
+      }
+    }
+  }
+  const u64 at = R.prefix(mine, total);
+  const u64 goal = min64(static_cast<u64>(u * static_cast<double>(total)), total - 1);
+  // The thread whose run holds the goal; its warp walks the run.
+  const uint32_t owner = __ballot_sync(0xffffffffu, at <= goal && goal < at + mine);
+  if (owner != 0) {
+    const int o = __ffs(static_cast<int>(owner)) - 1, lane = tid & 31;
+    const int w0 = __shfl_sync(0xffffffffu, i0, o), w1 = __shfl_sync(0xffffffffu, i1, o);
+    u64 base = __shfl_sync(0xffffffffu, at, o), tie = __shfl_sync(0xffffffffu, rank_of_tie, o);
+    for (int i = w0; i < w1; i += 32) {
+      const float v = i + lane < w1 ? elem(x, i + lane) : -INFINITY;
+      const uint32_t key = order_key(v);
+      const uint32_t ties = __ballot_sync(0xffffffffu, i + lane < w1 && key == cut_key);
+      const bool out = i + lane >= w1 || key < cut_key ||
+                       (key == cut_key && tie + __popc(ties & ((1u << lane) - 1)) >= cut_ties);
+      u64 w = out ? 0 : weight(v);
+      if (w < least) w = 0;
+      u64 inc = w;
+#pragma unroll
+      for (int s = 1; s < 32; s <<= 1) {
+        const u64 nb = __shfl_up_sync(0xffffffffu, inc, s);
+        if (lane >= s) inc += nb;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, goal < base + inc);
+      if (hit != 0) {
+        if (lane == __ffs(static_cast<int>(hit)) - 1) {
+          p.token[row] = first + i + lane;
+          if (p.logprob) p.logprob[row] = static_cast<float>(log(static_cast<double>(w) / static_cast<double>(total)));
+        }
         break;
       }
-      at += w;
+      base += __shfl_sync(0xffffffffu, inc, 31);
+      tie += __popc(ties);
     }
   }
   if (ranks > 1) cluster_sync_all();  // no CTA leaves while another reads its shared memory
 }
 
-template <class E>
-int launch_typed(SampleArgs p, int64_t B, cudaStream_t stream) {
+template <class E, int kThreads>
+int launch_typed(SampleArgs p, int64_t B, int64_t c, cudaStream_t stream) {
   int dev = 0;
   KW8_CUDA_TRY(cudaGetDevice(&dev));
   static std::atomic<uint64_t> attr_set{0};
   const uint64_t bit = 1ull << (dev & 63);
-  constexpr int kMaxSmem = 232448;
   if (!(attr_set.load() & bit)) {
-    KW8_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<E>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
+    KW8_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<E, kThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
+    KW8_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<E, kThreads>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     attr_set.fetch_or(bit);
   }
-  // CTAs per row: eight while the rows leave SMs idle, then as few as hold a row with two CTAs on an SM.
-  const int64_t fit = (110 * 1024 - static_cast<int64_t>(sizeof(SampShared))) / static_cast<int64_t>(sizeof(E));
-  int64_t c = (p.V + fit - 1) / fit;
-  c = std::max<int64_t>(c, std::min<int64_t>(8, (2 * 148 + B - 1) / B));
-  c = std::min<int64_t>(std::min<int64_t>(c, 8), std::max<int64_t>(1, p.V / 1024));
   p.slice = static_cast<int>((p.V + c - 1) / c);
-  const size_t smem = sizeof(SampShared) + static_cast<size_t>(p.slice) * sizeof(E);
-  KW8_REQUIRE(smem <= static_cast<size_t>(kMaxSmem), KW8_ERR_UNSUPPORTED, "vocabulary of %d too large", p.V);
+  const size_t smem = sizeof(SampShared) + static_cast<size_t>(p.slice) * sizeof(E) + 16;
+  KW8_REQUIRE(p.slice <= 65535 && smem <= static_cast<size_t>(kMaxSmem), KW8_ERR_UNSUPPORTED,
+              "vocabulary of %d too large", p.V);
   KW8_REQUIRE(B * c < (1ll << 31), KW8_ERR_UNSUPPORTED, "too many rows");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(B * c), 1, 1);
-  cfg.blockDim = dim3(kSampThreads, 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -431,16 +841,35 @@ int launch_typed(SampleArgs p, int64_t B, cudaStream_t stream) {
   attr[0].val.clusterDim.x = static_cast<unsigned>(c);
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = c > 1 ? 1 : 0;
-  KW8_CUDA_TRY(cudaLaunchKernelEx(&cfg, sample_kernel<E>, p));
+  cfg.numAttrs = 1;
+  KW8_CUDA_TRY(cudaLaunchKernelEx(&cfg, sample_kernel<E, kThreads>, p));
   return KW8_OK;
+}
+
+// CTAs per row: a power of two up to sixteen (other sizes pack badly into the
+// GPCs: 64 rows of 151936 bf16, top-k 50: 4 CTAs 23 us, 5 to 8 35 to 41 us).
+// One CTA per SM while every row has the same settings: a second one next to it
+// costs more in exchanges than it gains (256 x 32000 bf16: 1 CTA a row 20 us, 2
+// 30 us).  With settings of one per row the slowest rows bound the launch, and
+// up to four waves of smaller CTAs even them out (64 x 151643 fp32: 4 CTAs a
+// row 85 us, 8 69 us).
+template <class E>
+int launch_split(const SampleArgs& p, int64_t B, cudaStream_t stream) {
+  const bool per_row = p.temperature || p.top_k || p.top_p || p.min_p;
+  const int64_t most = per_row ? 4 * 148 : 148;
+  int64_t c = per_row ? 8 : 16;
+  while (c > 1 && (c * B > most || p.V / c < 2048)) c /= 2;
+  const int64_t fit = std::min<int64_t>(
+      65535, (kMaxSmem - 16 - static_cast<int64_t>(sizeof(SampShared))) / static_cast<int64_t>(sizeof(E)));
+  while (c < 8 && c * fit < p.V) c *= 2;
+  return launch_typed<E, 512>(p, B, c, stream);
 }
 
 }  // namespace
 
 int launch_sample(const SampleArgs& args, int64_t B, int logits_dtype, cudaStream_t stream) {
-  return logits_dtype == KW8_DT_F32 ? launch_typed<float>(args, B, stream)
-                                    : launch_typed<__nv_bfloat16>(args, B, stream);
+  return logits_dtype == KW8_DT_F32 ? launch_split<float>(args, B, stream)
+                                    : launch_split<__nv_bfloat16>(args, B, stream);
 }
 
 }  // namespace kw8
