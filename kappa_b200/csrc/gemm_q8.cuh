@@ -28,7 +28,6 @@ struct Q8LinearArgs {
   int stages;      // ring depth
   int k_splits;    // CTAs of a cluster that share one tile's k range
   int w_tiled;     // weights in the tiled layout
-  int tile_ftiles;
 };
 
 int launch_linear_q8(const int8_t* q, const kw8_weight& w, const Q8LinearArgs& args, cudaStream_t stream);

@@ -65,6 +65,24 @@ def test_packed_weights_give_the_same_bits(T, K, N):
         assert torch.equal(qlin.linear_q8(x, pack_weight(w, in_axis=-1), out_dtype=dtype), _ref(x, w, dtype))
 
 
+@pytest.mark.parametrize("T,K,N", [(300, 64, 1), (300, 64, 3), (257, 64, 63), (257, 64, 65), (270, 80, 127), (513, 64, 255), (258, 64, 258),
+                                   (400, 48, 301)])
+def test_widths_around_the_tiles(T, K, N):
+    """Output rows that start at every alignment, ends inside a word, a box and a tile."""
+    x, w = _rows(T, K, N), _weight(N, K, N)
+    for dtype in (torch.bfloat16, torch.float32):
+        buf = torch.full((T * N + 8,), 7.0, dtype=dtype, device="cuda")
+        for shift in (0, 1, 4):
+            out = buf[shift:shift + T * N].reshape(T, N)
+            wk = _lib.KW8Weight(w.values.data_ptr(), w.scale.data_ptr(), _lib.DT_F32, 1, 0, 0)
+            _lib.check(_lib.load().kw8_linear_q8(x.values.data_ptr(), x.scale.data_ptr(), T, K, N, wk,
+                                                 _lib.DT_F32 if dtype == torch.float32 else _lib.DT_BF16, out.data_ptr(),
+                                                 _lib.stream_of(out)))
+            assert torch.equal(out, _ref(x, w, dtype))
+            assert (buf[:shift] == 7).all() and (buf[shift + T * N:] == 7).all()
+            buf.fill_(7.0)
+
+
 def test_largest_sums():
     """Every product at its extreme: the sum reaches 128 * 128 * K just below 2^31."""
     K = 131056
