@@ -8,6 +8,9 @@ from kappa_b200 import _lib
 from kappa_b200.qwen3.quant import KMajor, Q8Rows, check_rows
 
 
+_OUT_DT = {torch.bfloat16: _lib.DT_BF16, torch.float32: _lib.DT_F32}
+
+
 def check_x(x: torch.Tensor, d: int | None = None) -> None:
     _lib.require_cuda(x, "x")
     if x.dim() != 3:
@@ -95,26 +98,35 @@ def linear_q8(x: Q8Rows, w: KMajor, *, out_dtype: torch.dtype = torch.bfloat16) 
 
     Returns ``[.., N]``, N over all leading axes of ``w``.
     """
-    if out_dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"out_dtype must be bfloat16 or float32, got {out_dtype}")
-    check_rows(x)
-    v = x.values
-    K = int(w.shape[-1])
-    if int(v.shape[-1]) != K:
-        raise ValueError(f"x rows have {int(v.shape[-1])} features, the weight takes {K}")
-    if w.layout == _lib.LAYOUT_TILED and len(w.shape) > 2 and int(w.shape[-2]) % 16:
+    if w.layout == _lib.LAYOUT_TILED and len(w.shape) > 2 and w.shape[-2] % 16:
         raise ValueError("a stacked tiled weight is one linear layer only when its rows per group are a multiple of 16")
-    if w.q.device != v.device:
-        raise ValueError(f"x is on {v.device}, the weight on {w.q.device}")
     N = 1
     for d in w.shape[:-1]:
         N *= d
-    with _lib.on_device(v):
-        vc, sc = v.contiguous(), x.scale.contiguous()
-        if vc.data_ptr() % 16:
-            vc = vc.clone()
-        out = vc.new_empty(v.shape[:-1] + (N,), dtype=out_dtype)
-        _lib.check(_lib.load().kw8_linear_q8(
-            vc.data_ptr(), sc.data_ptr(), vc.numel() // K, K, N, w.struct(),
-            _lib.DT_F32 if out_dtype == torch.float32 else _lib.DT_BF16, out.data_ptr(), _lib.stream_of(vc)))
+    return linear_q8_rows(x, w.struct(), w.q, N, w.shape[-1], out_dtype)
+
+
+def linear_q8_rows(x: Q8Rows, w: _lib.KW8Weight, wq: torch.Tensor, N: int, K: int, out_dtype: torch.dtype) -> torch.Tensor:
+    """``linear_q8`` of a weight given as its kw8_weight (values in ``wq``) and K-major shape ``[N, K]``."""
+    check_rows(x)
+    v, s = x
+    if _lib.elsewhere(v):
+        with torch.cuda.device(v.device):
+            return linear_q8_rows(x, w, wq, N, K, out_dtype)
+    dt = _OUT_DT.get(out_dtype)
+    if dt is None:
+        raise ValueError(f"out_dtype must be bfloat16 or float32, got {out_dtype}")
+    shape = v.shape
+    if shape[-1] != K:
+        raise ValueError(f"x rows have {shape[-1]} features, the weight takes {K}")
+    if wq.get_device() != v.get_device():
+        raise ValueError(f"x is on {v.device}, the weight on {wq.device}")
+    vc, sc = v.contiguous(), s.contiguous()
+    if vc.data_ptr() % 16:
+        vc = vc.clone()
+    out = vc.new_empty(shape[:-1] + (N,), dtype=out_dtype)
+    code = _lib.load().kw8_linear_q8(vc.data_ptr(), sc.data_ptr(), vc.numel() // K, K, N, w, dt, out.data_ptr(),
+                                     _lib.stream_of(vc))
+    if code:
+        _lib.check(code)
     return out

@@ -7,7 +7,6 @@ missing, or no CUDA device is present, calls raise.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import threading
@@ -284,14 +283,12 @@ def stream_of(t: torch.Tensor) -> int:
     return _raw_stream(t.device.index)
 
 
-def on_device(t: torch.Tensor):
-    """Context in which ``t``'s device is the current one (kernels launch on the current device)."""
-    if t.device.index == torch.cuda.current_device():
-        return _HERE
-    return torch.cuda.device(t.device)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-_HERE = contextlib.nullcontext()
+def elsewhere(t: torch.Tensor) -> bool:
+    """Whether CUDA tensor ``t`` is on another device than the current one (kernels launch on the current device)."""
+    return t.get_device() != _current_device()
 
 
 def device_status(t: torch.Tensor) -> int:

@@ -42,37 +42,42 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, scale: torch.Te
     ``h`` is ``x`` itself when there is no residual.
     """
     _lib.require_cuda(x, "x")
+    if _lib.elsewhere(x):
+        with torch.cuda.device(x.device):
+            return add_rms_norm(x, residual, scale, kind=kind, epsilon=epsilon, quantize=quantize)
     if x.dtype != torch.bfloat16:
         raise ValueError(f"x must be bfloat16 (the W8 path computes in bf16), got {x.dtype}")
-    if x.dim() < 1:
+    shape = x.shape
+    if not shape:
         raise ValueError("x must have a feature axis")
-    dev = x.device
+    dev, d = x.get_device(), shape[-1]
+    xc = _rows(x)
+    r_ptr = h_ptr = None
+    h = x
     if residual is not None:
         _lib.require_cuda(residual, "residual")
-        if residual.dtype != torch.bfloat16 or residual.shape != x.shape or residual.device != dev:
-            raise ValueError(f"residual must be bfloat16 {tuple(x.shape)} on {dev}, got {residual.dtype} "
+        if residual.dtype != torch.bfloat16 or residual.shape != shape or residual.get_device() != dev:
+            raise ValueError(f"residual must be bfloat16 {tuple(shape)} on {x.device}, got {residual.dtype} "
                              f"{tuple(residual.shape)} on {residual.device}")
-    d = int(x.shape[-1])
+        rc = _rows(residual)
+        h = torch.empty_like(xc)
+        r_ptr, h_ptr = rc.data_ptr(), h.data_ptr()
     s = _scale(scale, d, "scale")
-    if s.device != dev:
-        raise ValueError(f"scale is on {s.device}, x on {dev}")
-    with _lib.on_device(x):
-        xc = _rows(x)
-        rc = None if residual is None else _rows(residual)
-        h = x if rc is None else torch.empty_like(xc)
-        y = q = qs = None
-        if quantize:
-            q = torch.empty_like(xc, dtype=torch.int8)
-            qs = xc.new_empty(xc.shape[:-1] + (1,), dtype=torch.float32)
-            out = (None, q.data_ptr(), qs.data_ptr())
-        else:
-            y = torch.empty_like(xc)
-            out = (y.data_ptr(), None, None)
-        T = xc.numel() // d if d else 0
-        _lib.check(_lib.load().kw8_add_rms_norm(
-            xc.data_ptr(), None if rc is None else rc.data_ptr(), T, d, s.data_ptr(), _SCALE_DT[s.dtype], kind, epsilon,
-            None if rc is None else h.data_ptr(), *out, _lib.stream_of(xc)))
-    return h, (Q8Rows(q, qs) if quantize else y)
+    if s.get_device() != dev:
+        raise ValueError(f"scale is on {s.device}, x on {x.device}")
+    if quantize:
+        q = torch.empty_like(xc, dtype=torch.int8)
+        qs = xc.new_empty(shape[:-1] + (1,), dtype=torch.float32)
+        y, y_ptr, q_ptr, qs_ptr = Q8Rows(q, qs), None, q.data_ptr(), qs.data_ptr()
+    else:
+        y = torch.empty_like(xc)
+        y_ptr, q_ptr, qs_ptr = y.data_ptr(), None, None
+    code = _lib.load().kw8_add_rms_norm(xc.data_ptr(), r_ptr, xc.numel() // d if d else 0, d, s.data_ptr(),
+                                       _SCALE_DT[s.dtype], kind, epsilon, h_ptr, y_ptr, q_ptr, qs_ptr,
+                                       _lib.stream_of(xc))
+    if code:
+        _lib.check(code)
+    return h, y
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:

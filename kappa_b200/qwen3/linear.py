@@ -21,7 +21,7 @@ from __future__ import annotations
 
 import torch
 
-from kappa_b200 import _dense
+from kappa_b200 import _dense, _lib
 from kappa_b200.qwen3.quant import KMajor, Q8Rows, Q8Weight, Weight, is_q8_weight, kmajor, quantize_weight
 
 __all__ = ["project_q", "project_kv", "project_attn_out", "quantize_attn_out", "attn_out_kmajor",
@@ -36,6 +36,16 @@ def linear_q8(x: Q8Rows, w: Weight, *, in_axis: int = -1, out_dtype: torch.dtype
     """
     if not isinstance(x, Q8Rows):
         raise TypeError("x: linear_q8 takes 8-bit rows (add_rms_norm_q8, rms_norm_q8)")
+    if type(w) is Q8Weight and in_axis == -1:
+        # A weight [N, K] as it is stored: no views to make (kmajor's take as long as the launch).
+        q, s = w
+        if (q.is_cuda and q.dtype is torch.int8 and q.dim() == 2 and q.is_contiguous() and s.is_contiguous()
+                and s.get_device() == q.get_device()):
+            N, K = q.shape
+            n, dt = s.numel(), _dense._OUT_DT.get(s.dtype)
+            if dt is not None and (n == 1 or n == N):
+                weight = _lib.KW8Weight(q.data_ptr(), s.data_ptr(), dt, 1 if n > 1 else 0, _lib.LAYOUT_KMAJOR, 0)
+                return _dense.linear_q8_rows(x, weight, q, N, K, out_dtype)
     return _dense.linear_q8(x, kmajor(w, in_axis, "w"), out_dtype=out_dtype)
 
 

@@ -273,29 +273,35 @@ def to_compute_dtype(w: Weight, dtype: torch.dtype, *, in_axis: int = -2) -> tor
 
 def check_rows(x: Q8Rows, name: str = "x") -> None:
     """``x`` is a ``Q8Rows`` of CUDA tensors of one device with one scale per row."""
-    v, s = x.values, x.scale
+    v, s = x
     _lib.require_cuda(v, name)
-    _lib.require_cuda(s, f"{name}.scale")
+    _lib.require_cuda(s, name)
     if v.dtype != torch.int8 or s.dtype != torch.float32:
         raise ValueError(f"{name}: 8-bit rows are int8 values with fp32 scales, got {v.dtype} and {s.dtype}")
-    if v.dim() < 1 or s.shape != v.shape[:-1] + (1,):
-        raise ValueError(f"{name}: values {tuple(v.shape)} need one scale per row, got {tuple(s.shape)}")
-    if s.device != v.device:
+    shape = v.shape
+    if not shape or s.shape != shape[:-1] + (1,):
+        raise ValueError(f"{name}: values {tuple(shape)} need one scale per row, got {tuple(s.shape)}")
+    if s.get_device() != v.get_device():
         raise ValueError(f"{name}: scale and values on different devices")
 
 
 def dequantize_rows(x: Q8Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values that 8-bit rows stand for: ``values * scale`` in fp32, rounded once to ``dtype``."""
     check_rows(x)
-    if dtype not in _DT:
+    v, s = x
+    if _lib.elsewhere(v):
+        with torch.cuda.device(v.device):
+            return dequantize_rows(x, dtype)
+    dt = _DT.get(dtype)
+    if dt is None:
         raise ValueError(f"dequantize_rows: unsupported dtype {dtype}")
-    v = x.values
-    d = int(v.shape[-1])
-    with _lib.on_device(v):
-        vc, sc = v.contiguous(), x.scale.contiguous()
-        out = torch.empty(v.shape, dtype=dtype, device=v.device)
-        _lib.check(_lib.load().kw8_dequantize_rows(vc.data_ptr(), sc.data_ptr(), vc.numel() // d if d else 0, d,
-                                                   _DT[dtype], out.data_ptr(), _lib.stream_of(v)))
+    d = v.shape[-1]
+    vc, sc = v.contiguous(), s.contiguous()
+    out = torch.empty_like(vc, dtype=dtype)
+    code = _lib.load().kw8_dequantize_rows(vc.data_ptr(), sc.data_ptr(), vc.numel() // d if d else 0, d, dt,
+                                           out.data_ptr(), _lib.stream_of(v))
+    if code:
+        _lib.check(code)
     return out
 
 

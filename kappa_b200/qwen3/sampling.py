@@ -19,7 +19,11 @@ __all__ = ["sample_tokens"]
 _DT = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16}
 
 
-def _setting(v, name: str, lead: torch.Size, device: torch.device, dtype: torch.dtype):
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _setting(v, name: str, lead: torch.Size, device: int, dtype: torch.dtype):
     """(the tensor of one value per row or None, the one value or 0)."""
     if not isinstance(v, torch.Tensor):
         if dtype == torch.int32:
@@ -29,9 +33,9 @@ def _setting(v, name: str, lead: torch.Size, device: torch.device, dtype: torch.
         if v != v:
             raise ValueError(f"{name} is NaN")
         return None, float(v)
-    if v.shape != lead or v.device != device:
-        raise ValueError(f"{name}: one value per row wants shape {tuple(lead)} on {device}, got {tuple(v.shape)} on "
-                         f"{v.device}")
+    if v.shape != lead or v.get_device() != device:
+        raise ValueError(f"{name}: one value per row wants shape {tuple(lead)} on cuda:{device}, got {tuple(v.shape)} "
+                         f"on {v.device}")
     if v.is_floating_point() != (dtype == torch.float32) or v.dtype == torch.bool:
         raise ValueError(f"{name}: unsupported dtype {v.dtype}")
     if dtype == torch.int32 and v.dtype == torch.int64:
@@ -65,25 +69,28 @@ def sample_tokens(
         raise ValueError(f"logits must be bfloat16 or float32, got {logits.dtype}")
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits must be [.., V], got {tuple(logits.shape)}")
-    lead, dev = logits.shape[:-1], logits.device
-    if u.dtype != torch.float32 or u.shape != lead or u.device != dev:
-        raise ValueError(f"u must be float32 {tuple(lead)} on {dev}, got {u.dtype} {tuple(u.shape)} on {u.device}")
-    V = int(logits.shape[-1])
-    with _lib.on_device(logits):
-        t, t0 = _setting(temperature, "temperature", lead, dev, torch.float32)
-        k, k0 = _setting(top_k, "top_k", lead, dev, torch.int32)
-        p, p0 = _setting(top_p, "top_p", lead, dev, torch.float32)
-        m, m0 = _setting(min_p, "min_p", lead, dev, torch.float32)
-        # Rows may be strided (the last positions of [B, T, V]); the vocabulary may not.
-        x = logits if logits.dim() == 2 else logits.reshape(-1, V)
-        if x.stride(-1) != 1 and V > 1:
-            x = x.contiguous()
-        B = int(x.shape[0])
-        uc = u.contiguous()
-        token = uc.new_empty(lead, dtype=torch.int32)
-        logprob = torch.empty_like(uc)
-        s = _lib.KW8Sampling(*(None if v is None else v.data_ptr() for v in (t, k, p, m)), t0, k0, p0, m0)
-        _lib.check(_lib.load().kw8_sample(
-            x.data_ptr(), _DT[x.dtype], B, V, x.stride(0) if B > 1 else V, uc.data_ptr(), ctypes.byref(s),
-            token.data_ptr(), logprob.data_ptr(), _lib.stream_of(x)))
+    if _lib.elsewhere(logits):
+        with torch.cuda.device(logits.device):
+            return sample_tokens(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    shape, dev = logits.shape, logits.get_device()
+    lead, V = shape[:-1], shape[-1]
+    if u.dtype != torch.float32 or u.shape != lead or u.get_device() != dev:
+        raise ValueError(f"u must be float32 {tuple(lead)} on {logits.device}, got {u.dtype} {tuple(u.shape)} on {u.device}")
+    t, t0 = _setting(temperature, "temperature", lead, dev, torch.float32)
+    k, k0 = _setting(top_k, "top_k", lead, dev, torch.int32)
+    p, p0 = _setting(top_p, "top_p", lead, dev, torch.float32)
+    m, m0 = _setting(min_p, "min_p", lead, dev, torch.float32)
+    # Rows may be strided (the last positions of [B, T, V]); the vocabulary may not.
+    x = logits if len(shape) == 2 else logits.reshape(-1, V)
+    if V > 1 and x.stride(-1) != 1:
+        x = x.contiguous()
+    B = x.shape[0]
+    uc = u.contiguous()
+    token = torch.empty_like(uc, dtype=torch.int32)
+    logprob = torch.empty_like(uc)
+    settings = _lib.KW8Sampling(_ptr(t), _ptr(k), _ptr(p), _ptr(m), t0, k0, p0, m0)
+    code = _lib.load().kw8_sample(x.data_ptr(), _DT[x.dtype], B, V, x.stride(0) if B > 1 else V, uc.data_ptr(),
+                                  ctypes.byref(settings), token.data_ptr(), logprob.data_ptr(), _lib.stream_of(x))
+    if code:
+        _lib.check(code)
     return token, logprob
