@@ -233,7 +233,8 @@ int kw8_rms_norm(const void* x, int64_t T, int64_t D, const void* scale, int32_t
  * Exactly one of the two results is written; h_out (NULL: not stored) may
  * be x or residual itself, every other overlap is refused.
  *   x, residual, h_out, y_out: [T][D] bf16, 16-byte aligned; q_out [T][D]
- *   int8, 8-byte aligned; q_scale_out [T] fp32; D as for kw8_rms_norm.      */
+ *   int8, 8-byte aligned; q_scale_out [T] fp32; scale [D], 16-byte aligned;
+ *   D as for kw8_rms_norm.                                                   */
 int kw8_add_rms_norm(const void* x, const void* residual, int64_t T, int64_t D, const void* scale,
                      int32_t scale_dtype, int32_t kind, float eps, void* h_out, void* y_out,
                      int8_t* q_out, float* q_scale_out, kw8_stream_t stream);

@@ -62,7 +62,7 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, scale: torch.Te
         rc = _rows(residual)
         h = torch.empty_like(xc)
         r_ptr, h_ptr = rc.data_ptr(), h.data_ptr()
-    s = _scale(scale, d, "scale")
+    s = _rows(_scale(scale, d, "scale"))
     if s.get_device() != dev:
         raise ValueError(f"scale is on {s.device}, x on {x.device}")
     if quantize:

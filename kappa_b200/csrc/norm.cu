@@ -158,54 +158,41 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v, uint32_t* red, int tpr
   return v;
 }
 
-// Eight gains from d on: g = scale (+ 1 for Gemma).
-__device__ __forceinline__ void load_gain(const void* scale, int dtype, int kind, bool aligned, int64_t d,
-                                          float (&g)[8]) {
-  if (!aligned) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] = load_scale(scale, dtype, d + i);
-  } else if (dtype == KW8_DT_F32) {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(scale) + d);
-    const float4 a = __ldg(p), b = __ldg(p + 1);
-    g[0] = a.x; g[1] = a.y; g[2] = a.z; g[3] = a.w;
-    g[4] = b.x; g[5] = b.y; g[6] = b.z; g[7] = b.w;
-  } else {
-    bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(scale) + d)), g);
-  }
-  if (kind == KW8_NORM_GEMMA)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] += 1.0f;
+// The larger of a and |b|; NaN if either is.
+__device__ __forceinline__ float max_abs_nan(float a, float b) {
+  float d;
+  asm("{\n\t.reg .f32 t;\n\tabs.f32 t, %2;\n\tmax.NaN.f32 %0, %1, t;\n\t}" : "=f"(d) : "f"(a), "f"(b));
+  return d;
 }
 
 // Residual add + RMSNorm + optional 8-bit rows (definition in norm.cuh).
-// One pass: a row stays in its threads' registers (kVec 8-wide vectors per
+// One pass, a CTA per row: the row stays in its threads' registers (kVec 8-wide vectors per
 // thread at most) between the sum of squares, the absmax and the stores, so
-// each input is read once and each output written once; HBM is the bound.
-// The absmax is taken over the bit patterns of |y| (ordered like the values,
-// with infinity and NaN above every number), so one integer reduction also
-// finds the rows that are not finite.  Rounding to int8 is one fma:
-// y * (1/s) + 1.5 * 2^23 leaves the nearest integer (ties to even), in two's
-// complement, in the low byte of the sum's bits.  1/s rounds once, so a
-// value within about 2^-16 of a half step may round to the other side of it
-// than an exact division would.
-template <int kVec, bool kAdd, bool kQ8>
+// each input is read once and each output written once.  HBM is the bound, with
+// the issue slots close behind (about 13 instructions per value), hence the
+// shifts for divisions and 32-bit indexes inside a row.
+// The absmax keeps NaN (max.NaN), and its bit pattern is ordered like the value
+// with infinity and NaN above every number, so one integer reduction also finds
+// the rows that are not finite.  Rounding to int8 is one fma: y * (1/s) + 1.5 *
+// 2^23 leaves the nearest integer (ties to even), in two's complement, in the
+// low byte of the sum's bits.  1/s rounds once, so a value within about 2^-16 of
+// a half step may round to the other side of it than an exact division would.
+template <int kVec, bool kAdd, bool kQ8, bool kF32Gain>
 __global__ void __launch_bounds__(kNormThreads)
-    add_rms_norm_kernel(const uint4* x, const uint4* residual, int64_t T, int64_t D, const void* __restrict__ scale,
-                        int dtype, int kind, bool scale_aligned, float eps, int tpr, uint4* h_out, uint4* y_out,
-                        uint2* q_out, float* s_out) {
+    add_rms_norm_kernel(const uint4* x, const uint4* residual, int vec, const uint4* __restrict__ scale,
+                        float bias, float eps, int tpr_log2, uint4* h_out, uint4* y_out, uint2* q_out, float* s_out) {
   __shared__ float red[kNormThreads / 32];
   __shared__ uint32_t red_max[kNormThreads / 32];
-  const int64_t vec = D / 8;
-  const int tl = threadIdx.x % tpr;
-  const int64_t row = blockIdx.x * static_cast<int64_t>(blockDim.x / tpr) + threadIdx.x / tpr;
-  const int nv = row < T ? static_cast<int>((vec - tl + tpr - 1) / tpr) : 0;
+  const int tpr = 1 << tpr_log2, tl = static_cast<int>(threadIdx.x);
+  const int64_t row = blockIdx.x;
+  const int nv = (vec - tl + tpr - 1) >> tpr_log2;
   const int64_t e0 = row * vec + tl;
   uint4 a[kVec], b[kAdd ? kVec : 1];
 #pragma unroll
   for (int j = 0; j < kVec; ++j)
     if (j < nv) {
-      a[j] = x[e0 + j * tpr];
-      if constexpr (kAdd) b[j] = residual[e0 + j * tpr];
+      a[j] = (x + e0)[j << tpr_log2];
+      if constexpr (kAdd) b[j] = (residual + e0)[j << tpr_log2];
     }
   float ss = 0.f;
 #pragma unroll
@@ -219,33 +206,43 @@ __global__ void __launch_bounds__(kNormThreads)
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] += r[i];
         a[j] = f32x8_to_bf16(f);  // the residual stream is kept in bf16, and normed as it is kept
+        if (h_out != nullptr) (h_out + e0)[j << tpr_log2] = a[j];
         bf16x8_to_f32(a[j], f);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
     }
   const float total = group_sum(ss, red, tpr);
-  const float r = rsqrtf(__fdiv_rn(total, static_cast<float>(D)) + eps);
+  const float r = rsqrtf(__fdiv_rn(total, static_cast<float>(vec * 8)) + eps);
   float v[kVec][8];
-  uint32_t top = 0;
+  float top = 0.f;
 #pragma unroll
   for (int j = 0; j < kVec; ++j)
     if (j < nv) {
-      if (h_out != nullptr) h_out[e0 + j * tpr] = a[j];
+      if constexpr (!kAdd)
+        if (h_out != nullptr) (h_out + e0)[j << tpr_log2] = a[j];
       float g[8];
-      load_gain(scale, dtype, kind, scale_aligned, (static_cast<int64_t>(j) * tpr + tl) * 8, g);
+      if constexpr (kF32Gain) {
+        const uint4* p = scale + 2 * ((j << tpr_log2) + tl);
+        const uint4 lo = __ldg(p), hi = __ldg(p + 1);
+        const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = __uint_as_float(w[i]);
+      } else {
+        bf16x8_to_f32(__ldg(scale + (j << tpr_log2) + tl), g);
+      }
       bf16x8_to_f32(a[j], v[j]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        v[j][i] = __fmul_rn(__fmul_rn(v[j][i], r), g[i]);
-        if constexpr (kQ8) top = max(top, __float_as_uint(v[j][i]) & 0x7FFFFFFFu);
+        v[j][i] = __fmul_rn(__fmul_rn(v[j][i], r), g[i] + bias);  // g = scale + 1 (Gemma) or + 0
+        if constexpr (kQ8) top = max_abs_nan(top, v[j][i]);
       }
-      if constexpr (!kQ8) y_out[e0 + j * tpr] = f32x8_to_bf16(v[j]);
+      if constexpr (!kQ8) (y_out + e0)[j << tpr_log2] = f32x8_to_bf16(v[j]);
     }
   if constexpr (kQ8) {
-    top = group_max(top, red_max, tpr);
-    const bool finite = top < 0x7F800000u;
-    const float s = finite ? fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), 1.17549435e-38f)
+    const uint32_t bits = group_max(__float_as_uint(top), red_max, tpr);
+    const bool finite = bits < 0x7F800000u;
+    const float s = finite ? fmaxf(__fdiv_rn(__uint_as_float(bits), 127.0f), 1.17549435e-38f)
                            : __uint_as_float(0x7FC00000u);
     const float inv = __fdiv_rn(1.0f, s);
 #pragma unroll
@@ -257,9 +254,9 @@ __global__ void __launch_bounds__(kNormThreads)
         uint2 o;
         o.x = __byte_perm(__byte_perm(m[0], m[1], 0x0040), __byte_perm(m[2], m[3], 0x0040), 0x5410);
         o.y = __byte_perm(__byte_perm(m[4], m[5], 0x0040), __byte_perm(m[6], m[7], 0x0040), 0x5410);
-        q_out[e0 + j * tpr] = finite ? o : make_uint2(0u, 0u);
+        (q_out + e0)[j << tpr_log2] = finite ? o : make_uint2(0u, 0u);
       }
-    if (tl == 0 && row < T) s_out[row] = s;
+    if (tl == 0) s_out[row] = s;
   }
 }
 
@@ -336,19 +333,34 @@ int launch_block_finish(const float* part, int splits, int64_t split_stride, int
 
 namespace {
 
-template <int kVec>
-int launch_add_rms_norm_vec(const uint4* x, const uint4* residual, int64_t T, int64_t D, const void* scale,
-                            int scale_dtype, int kind, float eps, int tpr, uint4* h_out, uint4* y_out,
-                            uint2* q_out, float* s_out, cudaStream_t stream) {
-  const int64_t rpc = norm_rows_per_cta(T, tpr);
-  const unsigned grid = static_cast<unsigned>((T + rpc - 1) / rpc), block = static_cast<unsigned>(rpc * tpr);
-  const bool aligned = (reinterpret_cast<uintptr_t>(scale) & 15) == 0;
-  auto kernel = residual ? (q_out ? add_rms_norm_kernel<kVec, true, true> : add_rms_norm_kernel<kVec, true, false>)
-                         : (q_out ? add_rms_norm_kernel<kVec, false, true> : add_rms_norm_kernel<kVec, false, false>);
-  kernel<<<grid, block, 0, stream>>>(x, residual, T, D, scale, scale_dtype, kind, aligned, eps, tpr, h_out, y_out,
-                                     q_out, s_out);
+struct AddNormArgs {
+  const void *x, *residual, *scale;
+  int T, vec;
+  bool f32_gain;
+  float bias, eps;
+  int tpr_log2;
+  void *h_out, *y_out;
+  int8_t* q_out;
+  float* s_out;
+};
+
+template <int kVec, bool kAdd, bool kQ8>
+int launch_add_rms_norm_vec(const AddNormArgs& a, cudaStream_t stream) {
+  auto kernel = a.f32_gain ? add_rms_norm_kernel<kVec, kAdd, kQ8, true> : add_rms_norm_kernel<kVec, kAdd, kQ8, false>;
+  kernel<<<static_cast<unsigned>(a.T), 1u << a.tpr_log2, 0, stream>>>(static_cast<const uint4*>(a.x), static_cast<const uint4*>(a.residual), a.vec,
+                                     static_cast<const uint4*>(a.scale), a.bias, a.eps, a.tpr_log2,
+                                     static_cast<uint4*>(a.h_out), static_cast<uint4*>(a.y_out),
+                                     reinterpret_cast<uint2*>(a.q_out), a.s_out);
   KW8_CHECK_LAUNCH();
   return KW8_OK;
+}
+
+template <int kVec>
+int launch_add_rms_norm_any(const AddNormArgs& a, cudaStream_t stream) {
+  if (a.residual) return a.q_out ? launch_add_rms_norm_vec<kVec, true, true>(a, stream)
+                                 : launch_add_rms_norm_vec<kVec, true, false>(a, stream);
+  return a.q_out ? launch_add_rms_norm_vec<kVec, false, true>(a, stream)
+                 : launch_add_rms_norm_vec<kVec, false, false>(a, stream);
 }
 
 bool overlaps(const void* a, int64_t na, const void* b, int64_t nb) {
@@ -370,6 +382,8 @@ int launch_add_rms_norm(const void* x, const void* residual, int64_t T, int64_t 
                 reinterpret_cast<uintptr_t>(h_out) | reinterpret_cast<uintptr_t>(y_out)) & 15) == 0 &&
                   (reinterpret_cast<uintptr_t>(q_out) & 7) == 0 && (reinterpret_cast<uintptr_t>(s_out) & 3) == 0,
               KW8_ERR_UNSUPPORTED, "RMSNorm rows must be 16-byte aligned (int8 rows 8-byte)");
+  KW8_REQUIRE((reinterpret_cast<uintptr_t>(scale) & 15) == 0, KW8_ERR_UNSUPPORTED,
+              "the norm's scale must be 16-byte aligned");
   // Outputs: h over its own input element by element, or no overlap at all.
   const int64_t n2 = T * D * 2, out_bytes = q_out ? T * D : n2;
   const void* out = q_out ? static_cast<const void*>(q_out) : y_out;
@@ -381,15 +395,34 @@ int launch_add_rms_norm(const void* x, const void* residual, int64_t T, int64_t 
   bad = bad || overlaps(scale, scale_bytes, out, out_bytes) || overlaps(scale, scale_bytes, h_out, n2) ||
         overlaps(scale, scale_bytes, s_out, T * 4);
   KW8_REQUIRE(!bad, KW8_ERR_INVALID_ARG, "the norm's outputs overlap its inputs or one another");
-  const int tpr = norm_tpr(T, D);
-  const int64_t per = (D / 8 + tpr - 1) / tpr;  // 8-wide vectors per thread
-  auto go = per <= 1 ? launch_add_rms_norm_vec<1>
-                     : per <= 2 ? launch_add_rms_norm_vec<2>
-                                : per <= 4 ? launch_add_rms_norm_vec<4>
-                                           : per <= 5 ? launch_add_rms_norm_vec<5> : launch_add_rms_norm_vec<kNormMaxVec>;
-  return go(static_cast<const uint4*>(x), static_cast<const uint4*>(residual), T, D, scale, scale_dtype, kind, eps,
-            tpr, static_cast<uint4*>(h_out), static_cast<uint4*>(y_out), reinterpret_cast<uint2*>(q_out), s_out,
-            stream);
+  AddNormArgs a{};
+  a.x = x;
+  a.residual = residual;
+  a.scale = scale;
+  a.T = static_cast<int>(T);
+  a.vec = static_cast<int>(D / 8);
+  a.f32_gain = scale_dtype == KW8_DT_F32;
+  a.bias = kind == KW8_NORM_GEMMA ? 1.f : 0.f;
+  a.eps = eps;
+  a.h_out = h_out;
+  a.y_out = y_out;
+  a.q_out = q_out;
+  a.s_out = s_out;
+  // Threads per row: the fewest that hold it in five vectors each, more while
+  // the rows would keep few threads busy.  A row per CTA, so that no row waits
+  // for another's reductions (8192 x 2560 with residual to int8 rows: one row
+  // per CTA 27.1 us, four 27.8; without residual 17.5 against 19.5; 4096 x 2048:
+  // 12.3 against 13.2).
+  int tpr = 32;
+  while (tpr < kNormThreads && (a.vec + tpr - 1) / tpr > 5) tpr *= 2;
+  while (tpr < kNormThreads && tpr < a.vec && T * tpr < 148 * 896) tpr *= 2;
+  while ((1 << a.tpr_log2) < tpr) ++a.tpr_log2;
+  const int per = (a.vec + tpr - 1) / tpr;  // 8-wide vectors per thread
+  if (per <= 1) return launch_add_rms_norm_any<1>(a, stream);
+  if (per <= 2) return launch_add_rms_norm_any<2>(a, stream);
+  if (per <= 3) return launch_add_rms_norm_any<3>(a, stream);
+  if (per <= 5) return launch_add_rms_norm_any<5>(a, stream);
+  return launch_add_rms_norm_any<kNormMaxVec>(a, stream);
 }
 
 }  // namespace kw8

@@ -290,26 +290,36 @@ __global__ void __launch_bounds__(256)
   const float s = __ldg(scale + row);
   if constexpr (kVec) {
     const uint4* src = reinterpret_cast<const uint4*>(q + row * D);
-    for (int64_t j = lane; j < D / 16; j += 32) {
-      const uint4 v = __ldg(src + j);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-      float f[16];
+    const int n = static_cast<int>(D / 16);
+    constexpr int kAtOnce = 5;  // loads in flight per lane: a 2560-wide row
+    for (int j0 = lane; j0 < n; j0 += 32 * kAtOnce) {
+      uint4 v[kAtOnce];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) f[i] = static_cast<float>(static_cast<int8_t>(w[i / 4] >> (8 * (i % 4)))) * s;
-      if constexpr (kF32) {
-        float4* dst = reinterpret_cast<float4*>(static_cast<float*>(out) + row * D) + j * 4;
+      for (int u = 0; u < kAtOnce; ++u)
+        if (j0 + 32 * u < n) v[u] = __ldg(src + j0 + 32 * u);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dst[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
-      } else {
-        uint32_t o[8];
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int j = j0 + 32 * u;
+        if (j >= n) break;
+        const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+        float f[16];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-          o[i] = *reinterpret_cast<const uint32_t*>(&b);
+        for (int i = 0; i < 16; ++i) f[i] = static_cast<float>(static_cast<int8_t>(w[i / 4] >> (8 * (i % 4)))) * s;
+        if constexpr (kF32) {
+          float4* dst = reinterpret_cast<float4*>(static_cast<float*>(out) + row * D) + static_cast<int64_t>(j) * 4;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dst[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+        } else {
+          uint32_t o[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            o[i] = *reinterpret_cast<const uint32_t*>(&b);
+          }
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + row * D) + static_cast<int64_t>(j) * 2;
+          dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+          dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
         }
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + row * D) + j * 2;
-        dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-        dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
       }
     }
   } else {
@@ -329,7 +339,7 @@ int launch_dequantize_rows(const int8_t* q, const float* scale, int64_t T, int64
                            cudaStream_t stream) {
   KW8_REQUIRE(T >= 0 && D >= 0, KW8_ERR_INVALID_ARG, "bad shape (T=%lld D=%lld)", (long long)T, (long long)D);
   KW8_REQUIRE(out_dtype == KW8_DT_F32 || out_dtype == KW8_DT_BF16, KW8_ERR_INVALID_ARG, "bad out dtype");
-  KW8_REQUIRE(T < (1ll << 31), KW8_ERR_UNSUPPORTED, "too many rows");
+  KW8_REQUIRE(T < (1ll << 31) && D < (1ll << 31), KW8_ERR_UNSUPPORTED, "shape out of range");
   if (T == 0 || D == 0) return KW8_OK;
   KW8_REQUIRE(q && scale && out, KW8_ERR_INVALID_ARG, "null pointer");
   const bool f32 = out_dtype == KW8_DT_F32;

@@ -34,6 +34,7 @@ def _norm(x=P, residual=P + (1 << 16), T=4, D=64, scale=P + (1 << 17), dt=L.DT_F
     (dict(q=None, qs=None), L.KW8_ERR_INVALID_ARG, "either"),
     (dict(x=P + 8), L.KW8_ERR_UNSUPPORTED, "aligned"),
     (dict(q=P + (1 << 19) + 4), L.KW8_ERR_UNSUPPORTED, "aligned"),
+    (dict(scale=P + (1 << 17) + 8), L.KW8_ERR_UNSUPPORTED, "aligned"),
     (dict(h=P + 16), L.KW8_ERR_INVALID_ARG, "overlap"),
     (dict(q=P), L.KW8_ERR_INVALID_ARG, "overlap"),
     (dict(q=None, qs=None, y=P), L.KW8_ERR_INVALID_ARG, "overlap"),
