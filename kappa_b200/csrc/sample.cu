@@ -58,19 +58,19 @@ __device__ __forceinline__ float elem(const __nv_bfloat16* s, int i) { return __
 __device__ __forceinline__ void put(float* s, int i, float x) { s[i] = x; }
 __device__ __forceinline__ void put(__nv_bfloat16* s, int i, float x) { s[i] = __float2bfloat16_rn(x); }
 
-// The 16 / sizeof(E) values of a vector, cleaned, and back.
+// The 16 / sizeof(E) values of a vector and back.
 __device__ __forceinline__ void unpack(const uint4& v, float (&f)[4]) {
-  f[0] = clean(__uint_as_float(v.x));
-  f[1] = clean(__uint_as_float(v.y));
-  f[2] = clean(__uint_as_float(v.z));
-  f[3] = clean(__uint_as_float(v.w));
+  f[0] = __uint_as_float(v.x);
+  f[1] = __uint_as_float(v.y);
+  f[2] = __uint_as_float(v.z);
+  f[3] = __uint_as_float(v.w);
 }
 __device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    f[2 * i] = clean(__uint_as_float(w[i] << 16));
-    f[2 * i + 1] = clean(__uint_as_float(w[i] & 0xFFFF0000u));
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
   }
 }
 __device__ __forceinline__ uint4 pack(const float (&f)[4]) {
@@ -124,6 +124,7 @@ struct alignas(16) SampShared {
   u64 pub[2][kMaxRanks][3];  // every CTA's values of a cluster-wide reduction (alternating)
   u64 cut_before;            // sum in front of the cut's bin
   uint32_t cut_bin, cut_count;
+  uint32_t first_bin;           // of a top-p cut's window
   uint32_t listed;              // tokens of this CTA down to the cut (entries of `list` while they fit)
   uint32_t lists[kMaxRanks];    // every CTA's
 };
@@ -322,6 +323,44 @@ struct Row {
     __syncthreads();
   }
 
+  // From the counts alone: the bins between which the top_p cut must lie.  The
+  // weights of bin b are in 2^44 e^(-(b + 1.02) s) - 1 .. 2^44 e^(-(b - 0.02) s), s the
+  // bins' span (0.02: the roundings of the bin).  sh.first_bin: the first that it
+  // can lie in, sh.cut_bin: the first that it cannot lie behind (as it was, where
+  // the bounds do not tell).
+  __device__ __forceinline__ void bound_cut(double top_p) {
+    constexpr int kPer = kBins / kThreads;
+    constexpr double kSpan = static_cast<double>(kBinSpan) / (kBins - 1);
+    u64 lo[kPer], hi[kPer], slo = 0, shi = 0, all_lo, all_hi;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int b = threadIdx.x * kPer + j;
+      const double w = kOne * exp(-(b + 1.02) * kSpan);
+      lo[j] = sh.count_sum[b] * static_cast<u64>(fmax(floor(w) - 1.0, 0.0));
+      hi[j] = sh.count_sum[b] * static_cast<u64>(ceil(w * 1.0336));  // e^(1.04 s) = 1.03307
+      slo += lo[j];
+      shi += hi[j];
+    }
+    u64 at_lo = block_prefix(slo, all_lo), at_hi = block_prefix(shi, all_hi);
+    const double least = top_p * static_cast<double>(all_lo) * (1 - 1e-12), most = top_p * static_cast<double>(all_hi) * (1 + 1e-12);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const uint32_t b = threadIdx.x * kPer + j;
+      if (static_cast<double>(at_hi) < least && !(static_cast<double>(at_hi + hi[j]) < least)) sh.first_bin = b;
+      if (static_cast<double>(at_lo) < most && !(static_cast<double>(at_lo + lo[j]) < most)) sh.cut_bin = b;
+      at_lo += lo[j];
+      at_hi += hi[j];
+    }
+    __syncthreads();
+  }
+
+  // Tokens in the bins up to and with `bin`.
+  __device__ __forceinline__ u64 count_to(int bin) {
+    u64 c = 0;
+    for (int b = threadIdx.x; b <= bin; b += kThreads) c += sh.count_sum[b];
+    return block_reduce(c, [](u64 a, u64 b) { return a + b; });
+  }
+
   // a[0 .. size) into descending order; size a power of two.
   __device__ __forceinline__ void sort(u64* a, int size) {
     for (int len = 2; len <= size; len <<= 1)
@@ -344,7 +383,7 @@ __device__ __forceinline__ u64 min64(u64 a, u64 b) { return a < b ? a : b; }
 __device__ __forceinline__ u64 add64(u64 a, u64 b) { return a + b; }
 
 template <class E, int kThreads>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
     sample_kernel(const SampleArgs p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   SampShared& sh = *reinterpret_cast<SampShared*>(smem_raw);
@@ -374,10 +413,10 @@ __global__ void __launch_bounds__(kThreads)
   E* const x = aligned + lead;
   float best = -INFINITY;
   int best_at = -1;  // none above -inf yet
+  const int v0 = (lead + kVec - 1) / kVec, v1 = (lead + n) / kVec;  // whole vectors
+  const int head = min(n, v0 * kVec - lead), tail = max(head, v1 * kVec - lead);
   {
     const uint4* gsrc = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(src) & ~static_cast<uintptr_t>(15));
-    const int v0 = (lead + kVec - 1) / kVec, v1 = (lead + n) / kVec;
-    const int head = min(n, v0 * kVec - lead), tail = max(head, v1 * kVec - lead);
     constexpr int kUnroll = 8;
     for (int i = tid; i < head; i += kThreads) {  // fewer than kVec: one per thread
       const float f = clean(elem(src, i));
@@ -396,8 +435,10 @@ __global__ void __launch_bounds__(kThreads)
           unpack(v[j], f);
           const int i = (base + j * kThreads) * kVec;
 #pragma unroll
-          for (int e = 0; e < kVec; ++e)
+          for (int e = 0; e < kVec; ++e) {
+            f[e] = clean(f[e]);
             if (f[e] > best) best = f[e], best_at = i + e - lead;
+          }
           *reinterpret_cast<uint4*>(aligned + i) = pack(f);
         }
     }
@@ -422,6 +463,8 @@ __global__ void __launch_bounds__(kThreads)
   }
   const float top = key_value(static_cast<uint32_t>(best_all >> 32));
 
+  // Bound by the 64-bit pipe where every token is weighed: 13 operations, 14 to
+  // 16 cycles of an SM per warp, whatever the unrolling (256 rows of 32000: 12 us).
   // floor(2^44 exp(-d / temperature)), d = m - v, by Tang's table-driven
   // exponential: d in steps of ln2 / 32, 2^(-n/32) from the table, the rest (at
   // most ln2 / 64) by its series to the 6th power (error below 4e-18), rounded
@@ -460,22 +503,55 @@ __global__ void __launch_bounds__(kThreads)
     return static_cast<int>(__float_as_uint(__fmaf_rz(d, static_cast<float>(kBins - 1), 8388608.f)) & (kBins - 1));
   };
 
+  // The logit at bin position `at`, two steps of the format up or down, which
+  // covers its rounding: tokens above upper(b - 0.5) lie in bins below b, tokens of
+  // the bins up to b not below lower(b + 1.5).
+  const auto edge_key = [&](float at) { return order_key(clean(bin_top - at / static_cast<float>(kBins - 1) / bin_scale)); };
+  const auto upper = [&](float at) { return key_value(min(edge_key(at) + 2, 0xFF800000u)); };
+  const auto lower = [&](float at) { return key_value(max(edge_key(at), 0x00800001u) - 2); };
+
   const bool use_k = k > 0 && k < p.V, use_p = top_p < 1.f, use_m = min_p > 0.f;
   // w >= min_p 2^44 in whole numbers (the product is exact).
   const u64 least = use_m ? static_cast<u64>(ceil(static_cast<double>(min_p) * kOne)) : 0;
   const double u = fmin(fmax(static_cast<double>(p.u[row]), 0.0), 1.0);
 
+  // For sums in the order of the vocabulary each thread owns a run of
+  // neighbouring tokens.
+  const int run_len = ((n + kThreads - 1) / kThreads) | 1;  // odd: no bank conflicts
+  const int i0 = min(n, tid * run_len), i1 = min(n, i0 + run_len);
+  const auto over_run = [&](auto&& f) {
+#pragma unroll 4
+    for (int i = i0; i < i1; ++i) f(elem(x, i));
+  };
+  // Sum of this thread's tokens above run_top, in front of the window in which a
+  // mass cut lies: certain to stay, and summed already.
+  u64 run_sum = 0;
+  float run_top = INFINITY;
+
   // The cut of the general path: tokens above cut_key stay, of those at it the first cut_ties.
   uint32_t cut_key = 0;
   uint32_t cut_ties = 0xffffffffu, cut_all = 0xffffffffu;  // kept, and present
 
+  // f(value, index) for every token of the slice, in no order; go() ends it.
+  const auto for_each = [&](auto&& f, auto&& go) {
+    if (tid < head) f(elem(x, tid), tid);
+    if (tail + tid < n) f(elem(x, tail + tid), tail + tid);
+    for (int b = v0 + tid; b < v1 && go(); b += kThreads) {
+      float fv[kVec];
+      unpack(reinterpret_cast<const uint4*>(aligned)[b], fv);
+      const int i = b * kVec - lead;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) f(fv[e], i + e);
+    }
+  };
+  const auto always = [] { return true; };
   const auto count_all = [&] {
-#pragma unroll 8
-    for (int i = tid; i < n; i += kThreads) atomicAdd(&sh.count[bin_of(elem(x, i))], 1u);
+    for_each([&](float v, int) { atomicAdd(&sh.count[bin_of(v)], 1u); }, always);
   };
   if (use_k || use_p || use_m) {
     const bool mass = use_p && !use_k;
-    // The histogram that finds the first cut: of the masses, or of the counts.
+    // Counts find the bin of a top-k cut, and bound a top-p cut: a bin's weights
+    // differ by 3%, so the cut lies in a window of a few bins.
     // When at least top_k threads hold a token, the top_k-th largest of the
     // threads' own largest logits already bounds the cut (that many tokens are
     // not below it), at one addition per thread instead of one per token.
@@ -483,31 +559,22 @@ __global__ void __launch_bounds__(kThreads)
     double thr = 0.0;
     const bool by_threads = use_k && k <= kThreads * ranks / 2 && p.V >= kThreads * ranks;
     if (use_k || use_p) {
-      R.clear(mass);
-      if (mass) {
-        u64 sum = 0;
-#pragma unroll 8
-        for (int i = tid; i < n; i += kThreads) {
-          const float v = elem(x, i);
-          const u64 w = weight(v);
-          sum += w;
-          R.add_mass(bin_of(v), w);
-        }
-        R.sum(false, true);
-        sum = R.reduce(sum, add64);
-        thr = static_cast<double>(top_p) * static_cast<double>(sum);
-      } else {
-        if (by_threads) {
-          if (best_at >= 0) atomicAdd(&sh.count[bin_of(best)], 1u);
-        } else {
-          count_all();
-        }
-        R.sum(true, false);
-      }
+      R.clear(false);
+      if (!by_threads)
+        count_all();
+      else if (best_at >= 0)
+        atomicAdd(&sh.count[bin_of(best)], 1u);
+      R.sum(true, false);
       // Fewer threads than top_k above -inf: no bound, every token may be kept.
       sh.cut_bin = kBins - 1;
+      sh.first_bin = 0;
       __syncthreads();
-      R.find_cut(mass, static_cast<u64>(k), thr, 0);
+      if (use_k) {
+        R.find_cut(false, static_cast<u64>(k), 0.0, 0);
+      } else if (temp > 1e-31f && top < INFINITY) {  // elsewhere the bins are not linear in the logarithm
+        R.bound_cut(static_cast<double>(top_p));
+        if (sh.first_bin > 0) run_top = upper(static_cast<float>(sh.first_bin) - 0.5f);
+      }
       last = static_cast<int>(sh.cut_bin);
     }
     // w >= min_p 2^44 means (m - x) / temperature <= -ln min_p; two bins cover
@@ -515,23 +582,50 @@ __global__ void __launch_bounds__(kThreads)
     if (use_m && !(use_k && use_p))
       last = min(last, static_cast<int>(fminf(-logf(min_p) * ((kBins - 1) / kBinSpan), static_cast<float>(kBins))) + 2);
 
-    // Collect the tokens down to bin `last` as (key, ~index), as far as they fit.
-    // The bin as a bound on the logit: half a bin and two steps of the format
-    // lower, which covers the roundings (a few tokens too many do no harm).
-    const float low = bin_top - (static_cast<float>(last) + 1.5f) / static_cast<float>(kBins - 1) / bin_scale;
-    const uint32_t low_key = order_key(clean(low));
-    const float bound = low_key > 0x00800001u && last < kBins - 1 ? key_value(low_key - 2) : -INFINITY;
-    for (int base = tid; base < n; base += 8 * kThreads) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int i = base + j * kThreads;
-        const float v = elem(x, min(i, n - 1));
-        if (i < n && v >= bound) {
-          const uint32_t at = atomicAdd(&sh.listed, 1u);
-          if (at < kList) sh.list[at] = (static_cast<u64>(order_key(v)) << 32) | (0xffffffffu - static_cast<uint32_t>(first + i));
-        }
+    bool window = false;
+    if (mass) {
+      // All weights once: their sum, and where the list will not do (it reaches up
+      // to two bins further, see below) this thread's part of it in front of the
+      // window, and the window's own histogram.
+      window = R.count_to(min(last + 2, kBins - 1)) > kList;
+      u64 sum = 0;
+      if (!window) {
+        over_run([&](float v) { sum += weight(v); });
+      } else {
+        R.clear(true);
+        const int window_end = static_cast<int>(sh.cut_bin);
+        const float window_low = lower(static_cast<float>(window_end) + 1.5f);
+        over_run([&](float v) {
+          const u64 w = weight(v);
+          sum += w;
+          run_sum += v > run_top ? w : 0;
+          if (v <= run_top && v >= window_low) {
+            const int b = bin_of(v);
+            if (b <= window_end) R.add_mass(b, w);
+          }
+        });
       }
-      if (*static_cast<volatile uint32_t*>(&sh.listed) > kList) break;  // too many already
+      thr = static_cast<double>(top_p) * static_cast<double>(R.reduce(sum, add64));
+      if (window) {
+        R.sum(false, true);
+        R.find_cut(true, 0, thr, R.reduce(run_sum, add64));
+      }
+    }
+
+    // Collect the tokens down to bin `last` as (key, ~index), as far as they fit.
+    // The bin as a bound on the logit (a few tokens too many do no harm).
+    if (!window) {
+      const float bound = last < kBins - 1 ? lower(static_cast<float>(last) + 1.5f) : -INFINITY;
+      for_each(
+          [&](float v, int i) {
+            if (v >= bound) {
+              const uint32_t at = atomicAdd(&sh.listed, 1u);
+              if (at < kList) sh.list[at] = (static_cast<u64>(order_key(v)) << 32) | (0xffffffffu - static_cast<uint32_t>(first + i));
+            }
+          },
+          [&] { return *static_cast<volatile uint32_t*>(&sh.listed) <= kList; });  // not too many already
+    } else if (tid == 0) {
+      sh.listed = kList + 1;
     }
     __syncthreads();
     if (ranks > 1) {
@@ -672,29 +766,32 @@ __global__ void __launch_bounds__(kThreads)
       u64 before = sh.cut_before;
       const int bin = static_cast<int>(sh.cut_bin);
       u64 lo = 0xffffffffu, hi = 0, count = 0;
-      for (int i = tid; i < n; i += kThreads) {
-        const float v = elem(x, i);
-        if (bin_of(v) == bin) {
-          const uint32_t key = order_key(v);
-          lo = min64(lo, key);
-          hi = max64(hi, key);
-          ++count;
-        }
-      }
+      const float above = bin > 0 ? upper(static_cast<float>(bin) - 0.5f) : INFINITY, below = lower(static_cast<float>(bin) + 1.5f);
+      for_each(
+          [&](float v, int) {
+            if (v <= above && v >= below && bin_of(v) == bin) {
+              const uint32_t key = order_key(v);
+              lo = min64(lo, key);
+              hi = max64(hi, key);
+              ++count;
+            }
+          },
+          always);
       R.reduce3(lo, hi, count);
       while (lo != hi) {
         const int bits = 32 - __clz(static_cast<int>(hi - lo));
         const int shift = max(0, bits - 10);
         R.clear(by_mass);
-        for (int i = tid; i < n; i += kThreads) {
-          const float v = elem(x, i);
-          const uint32_t key = order_key(v);
-          if (key >= lo && key <= hi) {
-            const int b = static_cast<int>((hi - key) >> shift);
-            atomicAdd(&sh.count[b], 1u);
-            if (by_mass) R.add_mass(b, weight(v));
-          }
-        }
+        const float least_v = key_value(static_cast<uint32_t>(lo)), most_v = key_value(static_cast<uint32_t>(hi));
+        for_each(
+            [&](float v, int) {
+              if (v >= least_v && v <= most_v) {
+                const int b = static_cast<int>((hi - order_key(v)) >> shift);
+                atomicAdd(&sh.count[b], 1u);
+                if (by_mass) R.add_mass(b, weight(v));
+              }
+            },
+            always);
         R.sum(true, by_mass);
         R.find_cut(by_mass, goal_k, goal_p, before);
         before = sh.cut_before;
@@ -737,14 +834,16 @@ __global__ void __launch_bounds__(kThreads)
     if (use_k && use_p) {
       R.clear(true);
       u64 s = 0;
-      for (int i = tid; i < n; i += kThreads) {
-        const float v = elem(x, i);
-        if (order_key(v) >= cut_key) {
-          const u64 w = weight(v);
-          s += w;
-          R.add_mass(bin_of(v), w);
-        }
-      }
+      const float cut_v = cut_key == 0 ? -INFINITY : key_value(cut_key);
+      for_each(
+          [&](float v, int) {
+            if (v >= cut_v) {
+              const u64 w = weight(v);
+              s += w;
+              R.add_mass(bin_of(v), w);
+            }
+          },
+          always);
       s = R.reduce(s, add64);
       if (cut_ties < cut_all) s -= static_cast<u64>(cut_all - cut_ties) * ties_w;
       R.sum(false, true);
@@ -754,28 +853,29 @@ __global__ void __launch_bounds__(kThreads)
     }
   }
 
-  // The draw.  Each thread owns a run of neighbouring tokens.
-  const int run = ((n + kThreads - 1) / kThreads) | 1;  // odd: no bank conflicts
-  const int i0 = min(n, tid * run), i1 = min(n, i0 + run);
+  // The draw.
   u64 rank_of_tie = 0;
   if (cut_ties < cut_all) {
     u64 ties = 0, all;
-    for (int i = i0; i < i1; ++i) ties += order_key(elem(x, i)) == cut_key;
+    const float cut_v = key_value(cut_key);
+    for (int i = i0; i < i1; ++i) ties += elem(x, i) == cut_v;
     rank_of_tie = R.prefix(ties, all);
   }
   u64 mine = 0, total;
   if (cut_key == 0 && !use_m) {
-#pragma unroll 8
-    for (int i = i0; i < i1; ++i) mine += weight(elem(x, i));
+    over_run([&](float v) { mine += weight(v); });
   } else {
+    // What is summed already is not evaluated again (min_p may cut in front of the window).
+    const bool summed = run_top < INFINITY && !use_m;
+    const float cut_v = cut_key == 0 ? -INFINITY : key_value(cut_key);
+    if (summed) mine = run_sum;
     u64 tie = rank_of_tie;
     for (int i = i0; i < i1; ++i) {
       const float v = elem(x, i);
-      const uint32_t key = order_key(v);
-      if (key > cut_key || (key == cut_key && tie++ < cut_ties)) {
-        const u64 w = weight(v);
-        if (w >= least) mine += w;
-      }
+      if (v < cut_v || (summed && v > run_top)) continue;
+      if (v == cut_v && tie++ >= cut_ties) continue;
+      const u64 w = weight(v);
+      if (w >= least) mine += w;
     }
   }
   const u64 at = R.prefix(mine, total);
