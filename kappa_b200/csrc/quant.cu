@@ -277,9 +277,18 @@ int launch_dequantize(const kw8_weight& w, int64_t groups, int64_t N, int64_t K,
 
 namespace {
 
-// The values that 8-bit rows stand for.  A warp per row; with 16-byte
-// aligned rows (kVec) a lane reads 16 values at once.  HBM bound: D bytes
-// read and 2 D (4 D) written per row.
+// Four int8 values of a word in fp32, exactly: u = q + 128 placed in the low
+// byte of 2^23 makes the float 2^23 + u (the conversion instruction runs at a
+// quarter of this rate).
+__device__ __forceinline__ void i8x4_to_f32(uint32_t w, float (&f)[4]) {
+  const uint32_t u = w ^ 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 + i)) - 8388736.f;
+}
+
+// The values that 8-bit rows stand for.  A warp per row; with aligned rows
+// (kVec) a lane reads 8 values at once, so that a warp's loads and stores are
+// contiguous.  HBM bound: D bytes read and 2 D (4 D) written per row.
 template <bool kVec, bool kF32>
 __global__ void __launch_bounds__(256)
     dequantize_rows_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale, int64_t T, int64_t D,
@@ -289,11 +298,11 @@ __global__ void __launch_bounds__(256)
   if (row >= T) return;
   const float s = __ldg(scale + row);
   if constexpr (kVec) {
-    const uint4* src = reinterpret_cast<const uint4*>(q + row * D);
-    const int n = static_cast<int>(D / 16);
-    constexpr int kAtOnce = 5;  // loads in flight per lane: a 2560-wide row
+    const uint2* src = reinterpret_cast<const uint2*>(q + row * D);
+    const int n = static_cast<int>(D / 8);
+    constexpr int kAtOnce = 5;  // loads in flight per lane
     for (int j0 = lane; j0 < n; j0 += 32 * kAtOnce) {
-      uint4 v[kAtOnce];
+      uint2 v[kAtOnce];
 #pragma unroll
       for (int u = 0; u < kAtOnce; ++u)
         if (j0 + 32 * u < n) v[u] = __ldg(src + j0 + 32 * u);
@@ -301,24 +310,17 @@ __global__ void __launch_bounds__(256)
       for (int u = 0; u < kAtOnce; ++u) {
         const int j = j0 + 32 * u;
         if (j >= n) break;
-        const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-        float f[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = static_cast<float>(static_cast<int8_t>(w[i / 4] >> (8 * (i % 4)))) * s;
+        float lo[4], hi[4];
+        i8x4_to_f32(v[u].x, lo);
+        i8x4_to_f32(v[u].y, hi);
         if constexpr (kF32) {
-          float4* dst = reinterpret_cast<float4*>(static_cast<float*>(out) + row * D) + static_cast<int64_t>(j) * 4;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dst[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+          float4* dst = reinterpret_cast<float4*>(static_cast<float*>(out) + row * D) + static_cast<int64_t>(j) * 2;
+          dst[0] = make_float4(lo[0] * s, lo[1] * s, lo[2] * s, lo[3] * s);
+          dst[1] = make_float4(hi[0] * s, hi[1] * s, hi[2] * s, hi[3] * s);
         } else {
-          uint32_t o[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-            o[i] = *reinterpret_cast<const uint32_t*>(&b);
-          }
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + row * D) + static_cast<int64_t>(j) * 2;
-          dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-          dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+          alignas(16) const __nv_bfloat162 o[4] = {__floats2bfloat162_rn(lo[0] * s, lo[1] * s), __floats2bfloat162_rn(lo[2] * s, lo[3] * s),
+                                       __floats2bfloat162_rn(hi[0] * s, hi[1] * s), __floats2bfloat162_rn(hi[2] * s, hi[3] * s)};
+          reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + row * D)[j] = *reinterpret_cast<const uint4*>(o);
         }
       }
     }
@@ -346,7 +348,7 @@ int launch_dequantize_rows(const int8_t* q, const float* scale, int64_t T, int64
   KW8_REQUIRE((reinterpret_cast<uintptr_t>(out) & (f32 ? 3 : 1)) == 0 && (reinterpret_cast<uintptr_t>(scale) & 3) == 0,
               KW8_ERR_UNSUPPORTED, "misaligned rows");
   const bool vec =
-      D % 16 == 0 && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+      D % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   auto kernel = vec ? (f32 ? dequantize_rows_kernel<true, true> : dequantize_rows_kernel<true, false>)
                     : (f32 ? dequantize_rows_kernel<false, true> : dequantize_rows_kernel<false, false>);
   kernel<<<static_cast<unsigned>((T + 7) / 8), 256, 0, stream>>>(q, scale, T, D, out);
