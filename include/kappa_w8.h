@@ -199,7 +199,8 @@ int kw8_linear(const void* x, const int32_t* rows, int64_t T, int64_t K, int64_t
  *   q   : int8 [T][K], 16-byte aligned, K % 16 == 0, K <= 131056;
  *   q_scale: fp32 [T] (a NaN scale makes its row NaN);
  *   w   : one group, either layout; out: [T][N] in out_dtype.
- * No workspace; the result does not depend on how the work was split.       */
+ * No workspace; out overlaps no input; the result does not depend on how
+ * the work was split.                                                        */
 int kw8_linear_q8(const int8_t* q, const float* q_scale, int64_t T, int64_t K, int64_t N, kw8_weight w,
                   int32_t out_dtype, void* out, kw8_stream_t stream);
 

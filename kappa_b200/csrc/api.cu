@@ -958,7 +958,7 @@ int kw8_linear_q8(const int8_t* q, const float* q_scale, int64_t T, int64_t K, i
   KW8_REQUIRE(out_dtype == KW8_DT_BF16 || out_dtype == KW8_DT_F32, KW8_ERR_INVALID_ARG, "bad out dtype");
   KW8_REQUIRE(K % 16 == 0 && K <= kQ8MaxK, KW8_ERR_UNSUPPORTED,
               "K=%lld must be a multiple of 16 up to %lld (int32 sums)", (long long)K, (long long)kQ8MaxK);
-  KW8_REQUIRE(T < (1ll << 31) && N < (1ll << 31) - 256, KW8_ERR_UNSUPPORTED, "shape out of range");
+  KW8_REQUIRE(T < (1ll << 31) - 1024 && N < (1ll << 31) - 1024, KW8_ERR_UNSUPPORTED, "shape out of range");
   int rc = check_weight(w, "weight");
   if (rc || T == 0) return rc;
   KW8_REQUIRE(q && q_scale && out, KW8_ERR_INVALID_ARG, "null q/scale/out");
@@ -968,6 +968,11 @@ int kw8_linear_q8(const int8_t* q, const float* q_scale, int64_t T, int64_t K, i
                   (reinterpret_cast<uintptr_t>(w.scale) & (w.scale_dtype == KW8_DT_F32 ? 3 : 1)) == 0 &&
                   (reinterpret_cast<uintptr_t>(out) & (f32 ? 3 : 1)) == 0,
               KW8_ERR_UNSUPPORTED, "int8 operands must be 16-byte aligned, scales and out to their type");
+  const int64_t out_bytes = T * N * (f32 ? 4 : 2), w_scale_bytes = (w.per_channel ? N : 1) * (w.scale_dtype == KW8_DT_F32 ? 4 : 2);
+  const int64_t w_bytes = w.layout == KW8_LAYOUT_TILED ? tiled_bytes(1, N, K) : N * K;
+  KW8_REQUIRE(!overlaps(out, out_bytes, q, T * K) && !overlaps(out, out_bytes, q_scale, T * 4) &&
+                  !overlaps(out, out_bytes, w.q, w_bytes) && !overlaps(out, out_bytes, w.scale, w_scale_bytes),
+              KW8_ERR_INVALID_ARG, "out overlaps an input");
   Q8LinearArgs a{};
   a.T = static_cast<int>(T);
   a.N = static_cast<int>(N);
@@ -1029,6 +1034,16 @@ int kw8_sample(const void* logits, int32_t logits_dtype, int64_t B, int64_t V, i
                     reinterpret_cast<uintptr_t>(s->top_ks) | reinterpret_cast<uintptr_t>(s->top_ps) |
                     reinterpret_cast<uintptr_t>(s->min_ps)) & 3) == 0,
               KW8_ERR_UNSUPPORTED, "pointers must be aligned to their type");
+  const int64_t in_bytes = ((B - 1) * row_stride + V) * (logits_dtype == KW8_DT_F32 ? 4 : 2);
+  bool bad = overlaps(token_out, 4 * B, logprob_out, 4 * B);
+  for (const void* out : {static_cast<const void*>(token_out), static_cast<const void*>(logprob_out)}) {
+    bad = bad || overlaps(out, 4 * B, logits, in_bytes);
+    for (const void* in : {static_cast<const void*>(u), static_cast<const void*>(s->temperatures),
+                           static_cast<const void*>(s->top_ks), static_cast<const void*>(s->top_ps),
+                           static_cast<const void*>(s->min_ps)})
+      bad = bad || overlaps(out, 4 * B, in, 4 * B);
+  }
+  KW8_REQUIRE(!bad, KW8_ERR_INVALID_ARG, "an output overlaps an input or the other output");
   SampleArgs a{};
   a.logits = logits;
   a.ld = row_stride;

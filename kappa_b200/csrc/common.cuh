@@ -67,6 +67,12 @@ inline std::atomic<int> g_opt_ep_timing{0};
 
 // ----------------------------------------------------------- small utils --
 
+// Whether two ranges of bytes share one (null: no range).
+inline bool overlaps(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+  return a && b && p < q + static_cast<uintptr_t>(nb) && q < p + static_cast<uintptr_t>(na);
+}
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }

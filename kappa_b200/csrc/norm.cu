@@ -363,11 +363,6 @@ int launch_add_rms_norm_any(const AddNormArgs& a, cudaStream_t stream) {
                  : launch_add_rms_norm_vec<kVec, false, false>(a, stream);
 }
 
-bool overlaps(const void* a, int64_t na, const void* b, int64_t nb) {
-  const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
-  return a && b && p < q + static_cast<uintptr_t>(nb) && q < p + static_cast<uintptr_t>(na);
-}
-
 }  // namespace
 
 int launch_add_rms_norm(const void* x, const void* residual, int64_t T, int64_t D, const void* scale,

@@ -345,6 +345,9 @@ int launch_dequantize_rows(const int8_t* q, const float* scale, int64_t T, int64
   if (T == 0 || D == 0) return KW8_OK;
   KW8_REQUIRE(q && scale && out, KW8_ERR_INVALID_ARG, "null pointer");
   const bool f32 = out_dtype == KW8_DT_F32;
+  const int64_t out_bytes = T * D * (f32 ? 4 : 2);
+  KW8_REQUIRE(!overlaps(out, out_bytes, q, T * D) && !overlaps(out, out_bytes, scale, T * 4), KW8_ERR_INVALID_ARG,
+              "out overlaps an input");
   KW8_REQUIRE((reinterpret_cast<uintptr_t>(out) & (f32 ? 3 : 1)) == 0 && (reinterpret_cast<uintptr_t>(scale) & 3) == 0,
               KW8_ERR_UNSUPPORTED, "misaligned rows");
   const bool vec =

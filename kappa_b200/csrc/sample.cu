@@ -613,12 +613,13 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
 
     // Collect the tokens down to bin `last` as (key, ~index), as far as they fit.
-    // The bin as a bound on the logit (a few tokens too many do no harm).
+    // The bin as a bound on the logit (tokens of the two bins behind do no harm).
     if (!window) {
+      const int behind = min(last + 2, kBins - 1);
       const float bound = last < kBins - 1 ? lower(static_cast<float>(last) + 1.5f) : -INFINITY;
       for_each(
           [&](float v, int i) {
-            if (v >= bound) {
+            if (v >= bound && bin_of(v) <= behind) {
               const uint32_t at = atomicAdd(&sh.listed, 1u);
               if (at < kList) sh.list[at] = (static_cast<u64>(order_key(v)) << 32) | (0xffffffffu - static_cast<uint32_t>(first + i));
             }

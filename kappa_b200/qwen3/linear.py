@@ -96,6 +96,8 @@ def attn_out_kmajor(o_w: Weight) -> KMajor:
 
 def project_attn_out(encoded: torch.Tensor, o_w: Weight) -> torch.Tensor:
     """kappa/qwen3/linear.py:23-25: ``einsum("btnh,nhd->btd", encoded, o_w)``."""
+    if isinstance(encoded, Q8Rows):
+        raise TypeError("encoded: the output projection takes bf16 heads (8-bit rows: linear_q8 on attn_out_kmajor's weight)")
     km = attn_out_kmajor(o_w)
     d, nh = (int(s) for s in km.shape)
     if encoded.dim() != 4 or int(encoded.shape[2]) * int(encoded.shape[3]) != nh:

@@ -180,6 +180,31 @@ def test_values_over_the_whole_range():
             check(x, u, temperature=T, **kw)
 
 
+@pytest.mark.parametrize("offset,T", [(1e6, 1.0), (-1e6, 0.1), (3e7, 4.0), (1e5, 1e-3), (1e4, 30.0)])
+def test_logits_whose_steps_are_wider_than_a_bin(offset, T):
+    """Far from zero a step of the format spans several histogram bins, or a bin many tokens."""
+    for V in (3000, 40000):
+        g = torch.Generator(device="cuda").manual_seed(int(abs(offset)) + V)
+        x = torch.randn(3, V, generator=g, device="cuda") * 4 * T + offset
+        u = torch.rand(3, generator=g, device="cuda")
+        for kw in (dict(), dict(top_k=5), dict(top_k=700), dict(top_p=0.5), dict(top_p=0.97), dict(min_p=0.05),
+                   dict(top_p=0.9, min_p=0.3), dict(top_k=1500, top_p=0.8)):
+            check(x, u, temperature=T, **kw)
+
+
+@pytest.mark.parametrize("top_p", [0.01, 0.3, 0.7, 0.9, 0.99, 0.999999])
+@pytest.mark.parametrize("std", [0.0, 0.02, 0.5, 2.0, 8.0])
+def test_nuclei_of_every_width(top_p, std):
+    """From one token to nearly all: lists, windows of the histogram, and cuts among equal logits."""
+    for V, dtype in ((1500, torch.float32), (60000, torch.float32), (60000, torch.bfloat16)):
+        g = torch.Generator(device="cuda").manual_seed(int(100 * std) + V)
+        x = (torch.randn(3, V, generator=g, device="cuda") * std).to(dtype)
+        u = torch.rand(3, generator=g, device="cuda")
+        check(x, u, top_p=top_p)
+        check(x, u, top_p=top_p, min_p=0.2)
+        check(x, u, top_p=top_p, top_k=V // 2)
+
+
 def test_settings_that_are_not_numbers_take_the_first_token():
     x, u = make(4, 3000, 5)
     nan, one = torch.full((4,), math.nan, device="cuda"), torch.ones(4, device="cuda")

@@ -70,6 +70,10 @@ def _linear(q=P, qs=P + (1 << 16), T=4, K=64, N=32, w=None, dt=L.DT_BF16, out=P 
     (dict(q=P + 8), L.KW8_ERR_UNSUPPORTED, "aligned"),
     (dict(out=P + (1 << 18) + 1), L.KW8_ERR_UNSUPPORTED, "aligned"),
     (dict(out=P + (1 << 18) + 2, dt=L.DT_F32), L.KW8_ERR_UNSUPPORTED, "aligned"),
+    (dict(out=P), L.KW8_ERR_INVALID_ARG, "overlap"),
+    (dict(out=P + (1 << 17) + 64), L.KW8_ERR_INVALID_ARG, "overlap"),
+    (dict(out=P + (1 << 16)), L.KW8_ERR_INVALID_ARG, "overlap"),
+    (dict(out=P + (1 << 19)), L.KW8_ERR_INVALID_ARG, "overlap"),
     (dict(w=L.KW8Weight(None, P, L.DT_F32, 1, 0, 0)), L.KW8_ERR_INVALID_ARG, "null"),
     (dict(w=L.KW8Weight(P, P, 9, 1, 0, 0)), L.KW8_ERR_INVALID_ARG, "scale dtype"),
     (dict(w=L.KW8Weight(P, P, L.DT_F32, 1, 7, 0)), L.KW8_ERR_INVALID_ARG, "layout"),
@@ -117,6 +121,9 @@ NAN = float("nan")
     (dict(logits=P + 1, dt=L.DT_BF16), L.KW8_ERR_UNSUPPORTED, "aligned"),
     (dict(token=P + 2), L.KW8_ERR_UNSUPPORTED, "aligned"),
     (dict(temperatures=P + 1), L.KW8_ERR_UNSUPPORTED, "aligned"),
+    (dict(token=P + 1596), L.KW8_ERR_INVALID_ARG, "overlap"),
+    (dict(logprob=P + (1 << 17) + 12), L.KW8_ERR_INVALID_ARG, "overlap"),
+    (dict(logprob=P + (1 << 16)), L.KW8_ERR_INVALID_ARG, "overlap"),
 ])
 def test_sample_refuses(kw, code, text):
     assert _sample(**kw) == code
@@ -125,3 +132,27 @@ def test_sample_refuses(kw, code, text):
 
 def test_sample_of_no_rows_is_nothing():
     assert _sample(B=0, logits=None, u=None, token=None) == L.KW8_OK
+
+
+def _dequant(q=P, s=P + (1 << 16), T=4, D=64, dt=L.DT_BF16, out=P + (1 << 18)):
+    return L.load().kw8_dequantize_rows(q, s, T, D, dt, out, None)
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(q=None), L.KW8_ERR_INVALID_ARG, "null"),
+    (dict(s=None), L.KW8_ERR_INVALID_ARG, "null"),
+    (dict(out=None), L.KW8_ERR_INVALID_ARG, "null"),
+    (dict(T=-1), L.KW8_ERR_INVALID_ARG, "bad shape"),
+    (dict(T=1 << 31), L.KW8_ERR_UNSUPPORTED, "range"),
+    (dict(dt=3), L.KW8_ERR_INVALID_ARG, "dtype"),
+    (dict(out=P + (1 << 18) + 1), L.KW8_ERR_UNSUPPORTED, "misaligned"),
+    (dict(out=P + 128), L.KW8_ERR_INVALID_ARG, "overlap"),
+])
+def test_dequantize_rows_refuses(kw, code, text):
+    assert _dequant(**kw) == code
+    assert text in L.last_error()
+
+
+def test_dequantize_rows_of_nothing():
+    assert _dequant(T=0, q=None, s=None, out=None) == L.KW8_OK
+    assert _dequant(D=0, q=None, s=None, out=None) == L.KW8_OK
