@@ -263,7 +263,7 @@ typedef struct kw8_sampling {
 
 /* One token per row of logits, from given random numbers (kappa's sampling,
  * kappa/gemma3/sampling.py, draws its own).  Per row x, m = max x, a NaN logit
- * counting as -inf:
+ * counting as -inf and +inf as the largest finite number of its type:
  *   w_i = floor(2^44 * exp((x_i - m) / temperature)), exp in 64 bits;
  *   the tokens ordered by x descending, ties by index ascending;
  *   kept: the first top_k; of these the shortest prefix whose sum of w is at

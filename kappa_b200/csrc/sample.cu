@@ -1,6 +1,7 @@
 // Token sampling: temperature, top-k, top-p and min-p, from given random numbers.
 //
-// Per row of logits x (NaN counts as -inf), with m the largest:
+// Per row of logits x (NaN counts as -inf, +inf as the largest finite number),
+// with m the largest:
 //   w_i = floor(2^44 exp((x_i - m) / temperature)), a whole number, from a 64-bit exp;
 //   the tokens in the order (x descending, index ascending);
 //   kept: the first top_k of them; of these the shortest prefix whose sum of w
@@ -37,7 +38,7 @@ constexpr int kRanked = 256;      // up to here by counting, above by a sorting 
 constexpr int kMaxRanks = 16;
 constexpr int kMaxSmem = 232448;
 constexpr double kOne = 17592186044416.0;  // 2^44
-constexpr int kExpSteps = 32;         // table steps per octave of the exp (weight())
+constexpr int kExpSteps = 64, kExpCopies = 8;  // table steps per octave of the exp (weight()), copies side by side
 
 using u64 = unsigned long long;
 
@@ -50,8 +51,12 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
 }
 
-// NaN -> -inf, -0 -> +0.
-__device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY) + 0.0f; }
+// NaN -> -inf, +inf -> the largest finite number of the type, -0 -> +0.
+template <class E>
+__device__ __forceinline__ float clean(float x) {
+  constexpr float kMost = sizeof(E) == 4 ? 3.40282347e38f : 3.38953139e38f;
+  return fminf(fmaxf(x, -INFINITY), kMost) + 0.0f;
+}
 
 __device__ __forceinline__ float elem(const float* s, int i) { return s[i]; }
 __device__ __forceinline__ float elem(const __nv_bfloat16* s, int i) { return __bfloat162float(s[i]); }
@@ -119,7 +124,7 @@ struct alignas(16) SampShared {
     };
     u64 gathered[kList];
   };
-  double exp_table[kExpSteps * 16];  // 2^(-i / kExpSteps), sixteen copies side by side
+  double exp_table[kExpSteps * kExpCopies];  // 2^(44 - i / kExpSteps)
   u64 warp_a[32];
   u64 pub[2][kMaxRanks][3];  // every CTA's values of a cluster-wide reduction (alternating)
   u64 cut_before;            // sum in front of the cut's bin
@@ -401,7 +406,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   const float top_p = p.top_p ? p.top_p[row] : p.top_p0;
   const float min_p = p.min_p ? p.min_p[row] : p.min_p0;
   const int32_t k = p.top_k ? p.top_k[row] : p.top_k0;
-  for (int i = tid; i < kExpSteps * 16; i += kThreads) sh.exp_table[i] = exp2(-(i >> 4) * (1.0 / kExpSteps));
+  for (int i = tid; i < kExpSteps * kExpCopies; i += kThreads)
+    sh.exp_table[i] = exp2(44.0 - (i / kExpCopies) * (1.0 / kExpSteps));
   if (tid == 0) sh.listed = 0;
 
   // The slice into shared memory, at the alignment that it has in global
@@ -419,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const uint4* gsrc = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(src) & ~static_cast<uintptr_t>(15));
     constexpr int kUnroll = 8;
     for (int i = tid; i < head; i += kThreads) {  // fewer than kVec: one per thread
-      const float f = clean(elem(src, i));
+      const float f = clean<E>(elem(src, i));
       put(x, i, f);
       if (f > best) best = f, best_at = i;
     }
@@ -436,14 +442,14 @@ __global__ void __launch_bounds__(kThreads, 2)
           const int i = (base + j * kThreads) * kVec;
 #pragma unroll
           for (int e = 0; e < kVec; ++e) {
-            f[e] = clean(f[e]);
+            f[e] = clean<E>(f[e]);
             if (f[e] > best) best = f[e], best_at = i + e - lead;
           }
           *reinterpret_cast<uint4*>(aligned + i) = pack(f);
         }
     }
     for (int i = tail + tid; i < n; i += kThreads) {
-      const float f = clean(elem(src, i));
+      const float f = clean<E>(elem(src, i));
       put(x, i, f);
       if (f > best) best = f, best_at = i;
     }
@@ -463,50 +469,49 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   const float top = key_value(static_cast<uint32_t>(best_all >> 32));
 
-  // Bound by the 64-bit pipe where every token is weighed: 13 operations, 14 to
-  // 16 cycles of an SM per warp, whatever the unrolling (256 rows of 32000: 12 us).
   // floor(2^44 exp(-d / temperature)), d = m - v, by Tang's table-driven
-  // exponential: d in steps of ln2 / 32, 2^(-n/32) from the table, the rest (at
-  // most ln2 / 64) by its series to the 6th power (error below 4e-18), rounded
-  // down to 2^-44 in the bits.  No branches, so that several run at once; sixteen
-  // copies of the table, so that lanes do not meet in a bank.
+  // exponential: d in steps of ln2 / 64, 2^(44 - n/64) from the table (the octaves
+  // subtracted from the exponent), the rest (at most ln2 / 128) by its series to
+  // the 5th power (error below 4e-17), rounded down by adding 2^52.  No branches,
+  // so that several run at once; eight copies of the table, so that few lanes
+  // meet in a bank.  Where every token is weighed, the 64-bit pipe and the issue
+  // slots bound the kernel: 13 64-bit operations and about as many others, 10.5
+  // cycles of an SM per warp (with shifts and selects of 64-bit words instead of
+  // the additions 13.6), whatever the unrolling.
   const double top_d = static_cast<double>(top);
   const double per_step = kExpSteps * 1.4426950408889634 / static_cast<double>(temp);
   const uint32_t d_end = static_cast<uint32_t>(__double2hiint(46 * 0.6931471805599453 * static_cast<double>(temp)));
-  const double* const table = sh.exp_table + (tid & 15);
+  const double* const table = sh.exp_table + (tid & (kExpCopies - 1));
   const auto weight = [&](float v) -> u64 {
     constexpr double h = -0.6931471805599453 / kExpSteps;
     const double d = top_d - static_cast<double>(v);
     const double z = fma(d, per_step, 6755399441055744.0);  // 1.5 * 2^52: the low word is the nearest integer
     const double f = fma(d, per_step, 6755399441055744.0 - z);
     const int steps = __double2loint(z);
-    double e = fma(f, h * h * h * h * h * h / 720, h * h * h * h * h / 120);
-    e = fma(e, f, h * h * h * h / 24);
+    double e = fma(f, h * h * h * h * h / 120, h * h * h * h / 24);
     e = fma(e, f, h * h * h / 6);
     e = fma(e, f, h * h / 2);
     e = fma(e, f, h);
     e = fma(e, f, 1.0);
-    e *= table[(steps & (kExpSteps - 1)) * 16];
-    // e = (1.mantissa) 2^(exponent - 1023): 2^(44 - octaves) e rounded down is a shift.
-    const u64 bits = static_cast<u64>(__double_as_longlong(e));
-    const u64 w = ((bits & 0xFFFFFFFFFFFFFull) | 0x10000000000000ull) >>
-                  ((1031 - static_cast<int>(bits >> 52) + (steps >> 5)) & 63);
-    // From 46 octaves on, +inf and NaN (inf - inf, inf * 0) nothing is left.
+    e *= table[(steps & (kExpSteps - 1)) * kExpCopies];
+    // From 46 octaves on, and for -inf, nothing is left.
     const bool far = static_cast<uint32_t>(__double2hiint(d)) >= d_end;
-    return v == top ? 1ull << 44 : far ? 0 : w;
+    const int hi = far ? 0 : __double2hiint(e) - ((steps >> 6) << 20);
+    e = __dadd_rd(__hiloint2double(hi, __double2loint(e)), 4503599627370496.0);
+    return static_cast<u64>(__double_as_longlong(e)) & 0xFFFFFFFFFFFFFull;
   };
   // Monotone in v: a subtraction, a product cut to [0, 1], a product rounded
-  // down (by adding 2^23).  +inf on both sides gives -inf, bin 0.
-  const float bin_top = fminf(top, 3.4028235e38f), bin_scale = fminf(1.f / (kBinSpan * temp), 1e30f);
+  // down (by adding 2^23).
+  const float bin_scale = fminf(1.f / (kBinSpan * temp), 1e30f);
   const auto bin_of = [&](float v) -> int {
-    const float d = __saturatef((bin_top - v) * bin_scale);
+    const float d = __saturatef((top - v) * bin_scale);
     return static_cast<int>(__float_as_uint(__fmaf_rz(d, static_cast<float>(kBins - 1), 8388608.f)) & (kBins - 1));
   };
 
   // The logit at bin position `at`, two steps of the format up or down, which
   // covers its rounding: tokens above upper(b - 0.5) lie in bins below b, tokens of
   // the bins up to b not below lower(b + 1.5).
-  const auto edge_key = [&](float at) { return order_key(clean(bin_top - at / static_cast<float>(kBins - 1) / bin_scale)); };
+  const auto edge_key = [&](float at) { return order_key(top - at / static_cast<float>(kBins - 1) / bin_scale + 0.0f); };
   const auto upper = [&](float at) { return key_value(min(edge_key(at) + 2, 0xFF800000u)); };
   const auto lower = [&](float at) { return key_value(max(edge_key(at), 0x00800001u) - 2); };
 
@@ -571,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       __syncthreads();
       if (use_k) {
         R.find_cut(false, static_cast<u64>(k), 0.0, 0);
-      } else if (temp > 1e-31f && top < INFINITY) {  // elsewhere the bins are not linear in the logarithm
+      } else if (temp > 1e-31f) {  // below, the bins are not linear in the logarithm
         R.bound_cut(static_cast<double>(top_p));
         if (sh.first_bin > 0) run_top = upper(static_cast<float>(sh.first_bin) - 0.5f);
       }

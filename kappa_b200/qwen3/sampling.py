@@ -60,8 +60,8 @@ def sample_tokens(
     their probability, of these the ones at least ``min_p`` times as likely as
     the first.  The token is drawn from the kept ones in the order of their ids
     by ``u``, and the log-probability is its share of them.  ``temperature <=
-    0`` takes the first token (greedy).  NaN logits are never drawn; a row
-    without any logit above ``-inf`` gives token ``-1`` and ``-inf``.
+    0`` takes the first token (greedy).  NaN logits are never drawn, ``+inf``
+    counts as the largest finite number; a row without any logit above ``-inf`` gives token ``-1`` and ``-inf``.
     """
     _lib.require_cuda(logits, "logits")
     _lib.require_cuda(u, "u")
