@@ -58,8 +58,8 @@ __device__ __forceinline__ float clean(float x) {
   return fminf(fmaxf(x, -INFINITY), kMost) + 0.0f;
 }
 
-__device__ __forceinline__ float elem(const float* s, int i) { return s[i]; }
-__device__ __forceinline__ float elem(const __nv_bfloat16* s, int i) { return __bfloat162float(s[i]); }
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ void put(float* s, int i, float x) { s[i] = x; }
 __device__ __forceinline__ void put(__nv_bfloat16* s, int i, float x) { s[i] = __float2bfloat16_rn(x); }
 
@@ -387,7 +387,7 @@ __device__ __forceinline__ u64 max64(u64 a, u64 b) { return a > b ? a : b; }
 __device__ __forceinline__ u64 min64(u64 a, u64 b) { return a < b ? a : b; }
 __device__ __forceinline__ u64 add64(u64 a, u64 b) { return a + b; }
 
-template <class E, int kThreads>
+template <class E, int kThreads, bool kStaged>
 __global__ void __launch_bounds__(kThreads, 2)
     sample_kernel(const SampleArgs p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -410,25 +410,25 @@ __global__ void __launch_bounds__(kThreads, 2)
     sh.exp_table[i] = exp2(44.0 - (i / kExpCopies) * (1.0 / kExpSteps));
   if (tid == 0) sh.listed = 0;
 
-  // The slice into shared memory, at the alignment that it has in global
-  // memory (whole vectors inside, single values at the ends), and the row's
-  // first largest logit.
+  // The row's first largest logit.  The slice is read in whole vectors, with
+  // single values at its ends; kStaged: into shared memory, at the alignment that
+  // it has in global memory, else later passes find it in L1 and L2.
   constexpr int kVec = 16 / sizeof(E);
   const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(E));
+  const uint4* const gsrc = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(src) & ~static_cast<uintptr_t>(15));
   E* const aligned = reinterpret_cast<E*>(smem_raw + sizeof(SampShared));
-  E* const x = aligned + lead;
-  float best = -INFINITY;
-  int best_at = -1;  // none above -inf yet
   const int v0 = (lead + kVec - 1) / kVec, v1 = (lead + n) / kVec;  // whole vectors
   const int head = min(n, v0 * kVec - lead), tail = max(head, v1 * kVec - lead);
+  float best = -INFINITY;
+  int best_at = -1;  // none above -inf yet
   {
-    const uint4* gsrc = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(src) & ~static_cast<uintptr_t>(15));
-    constexpr int kUnroll = 8;
-    for (int i = tid; i < head; i += kThreads) {  // fewer than kVec: one per thread
-      const float f = clean<E>(elem(src, i));
-      put(x, i, f);
+    constexpr int kUnroll = 6;
+    const auto single = [&](int i) {
+      const float f = clean<E>(to_float(src[i]));
+      if constexpr (kStaged) put(aligned + lead, i, f);
       if (f > best) best = f, best_at = i;
-    }
+    };
+    if (tid < head) single(tid);
     for (int base = v0 + tid; base < v1; base += kUnroll * kThreads) {
       uint4 v[kUnroll];
 #pragma unroll
@@ -445,15 +445,19 @@ __global__ void __launch_bounds__(kThreads, 2)
             f[e] = clean<E>(f[e]);
             if (f[e] > best) best = f[e], best_at = i + e - lead;
           }
-          *reinterpret_cast<uint4*>(aligned + i) = pack(f);
+          if constexpr (kStaged) *reinterpret_cast<uint4*>(aligned + i) = pack(f);
         }
     }
-    for (int i = tail + tid; i < n; i += kThreads) {
-      const float f = clean<E>(elem(src, i));
-      put(x, i, f);
-      if (f > best) best = f, best_at = i;
-    }
+    if (tail + tid < n) single(tail + tid);
   }
+  // Token i of the slice.
+  const E* const x = kStaged ? aligned + lead : src;
+  const auto elem = [x](int i) -> float {
+    if constexpr (kStaged)
+      return to_float(x[i]);
+    else
+      return clean<E>(to_float(__ldg(x + i)));
+  };
   // (key, ~index): the largest value, of equals the lowest index.
   const u64 best_all = R.reduce(
       best_at < 0 ? 0 : (static_cast<u64>(order_key(best)) << 32) | (0xffffffffu - static_cast<uint32_t>(first + best_at)),
@@ -526,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int i0 = min(n, tid * run_len), i1 = min(n, i0 + run_len);
   const auto over_run = [&](auto&& f) {
 #pragma unroll 4
-    for (int i = i0; i < i1; ++i) f(elem(x, i));
+    for (int i = i0; i < i1; ++i) f(elem(i));
   };
   // Sum of this thread's tokens above run_top, in front of the window in which a
   // mass cut lies: certain to stay, and summed already.
@@ -539,14 +543,23 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   // f(value, index) for every token of the slice, in no order; go() ends it.
   const auto for_each = [&](auto&& f, auto&& go) {
-    if (tid < head) f(elem(x, tid), tid);
-    if (tail + tid < n) f(elem(x, tail + tid), tail + tid);
-    for (int b = v0 + tid; b < v1 && go(); b += kThreads) {
-      float fv[kVec];
-      unpack(reinterpret_cast<const uint4*>(aligned)[b], fv);
-      const int i = b * kVec - lead;
+    if (tid < head) f(elem(tid), tid);
+    if (tail + tid < n) f(elem(tail + tid), tail + tid);
+    constexpr int kAtOnce = kStaged ? 1 : 4;  // vectors in flight
+    for (int b = v0 + tid; b < v1 && go(); b += kAtOnce * kThreads) {
+      uint4 v[kAtOnce];
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) f(fv[e], i + e);
+      for (int j = 0; j < kAtOnce; ++j)
+        if (b + j * kThreads < v1) v[j] = kStaged ? reinterpret_cast<const uint4*>(aligned)[b] : __ldg(gsrc + b + j * kThreads);
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j)
+        if (b + j * kThreads < v1) {
+          float fv[kVec];
+          unpack(v[j], fv);
+          const int i = (b + j * kThreads) * kVec - lead;
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) f(kStaged ? fv[e] : clean<E>(fv[e]), i + e);
+        }
     }
   };
   const auto always = [] { return true; };
@@ -864,7 +877,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (cut_ties < cut_all) {
     u64 ties = 0, all;
     const float cut_v = key_value(cut_key);
-    for (int i = i0; i < i1; ++i) ties += elem(x, i) == cut_v;
+    for (int i = i0; i < i1; ++i) ties += elem(i) == cut_v;
     rank_of_tie = R.prefix(ties, all);
   }
   u64 mine = 0, total;
@@ -877,7 +890,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (summed) mine = run_sum;
     u64 tie = rank_of_tie;
     for (int i = i0; i < i1; ++i) {
-      const float v = elem(x, i);
+      const float v = elem(i);
       if (v < cut_v || (summed && v > run_top)) continue;
       if (v == cut_v && tie++ >= cut_ties) continue;
       const u64 w = weight(v);
@@ -893,7 +906,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int w0 = __shfl_sync(0xffffffffu, i0, o), w1 = __shfl_sync(0xffffffffu, i1, o);
     u64 base = __shfl_sync(0xffffffffu, at, o), tie = __shfl_sync(0xffffffffu, rank_of_tie, o);
     for (int i = w0; i < w1; i += 32) {
-      const float v = i + lane < w1 ? elem(x, i + lane) : -INFINITY;
+      const float v = i + lane < w1 ? elem(i + lane) : -INFINITY;
       const uint32_t key = order_key(v);
       const uint32_t ties = __ballot_sync(0xffffffffu, i + lane < w1 && key == cut_key);
       const bool out = i + lane >= w1 || key < cut_key ||
@@ -921,19 +934,19 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (ranks > 1) cluster_sync_all();  // no CTA leaves while another reads its shared memory
 }
 
-template <class E, int kThreads>
+template <class E, int kThreads, bool kStaged>
 int launch_typed(SampleArgs p, int64_t B, int64_t c, cudaStream_t stream) {
   int dev = 0;
   KW8_CUDA_TRY(cudaGetDevice(&dev));
   static std::atomic<uint64_t> attr_set{0};
   const uint64_t bit = 1ull << (dev & 63);
   if (!(attr_set.load() & bit)) {
-    KW8_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<E, kThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
-    KW8_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<E, kThreads>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    KW8_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<E, kThreads, kStaged>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
+    KW8_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<E, kThreads, kStaged>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     attr_set.fetch_or(bit);
   }
   p.slice = static_cast<int>((p.V + c - 1) / c);
-  const size_t smem = sizeof(SampShared) + static_cast<size_t>(p.slice) * sizeof(E) + 16;
+  const size_t smem = sizeof(SampShared) + (kStaged ? static_cast<size_t>(p.slice) * sizeof(E) + 16 : 0);
   KW8_REQUIRE(p.slice <= 65535 && smem <= static_cast<size_t>(kMaxSmem), KW8_ERR_UNSUPPORTED,
               "vocabulary of %d too large", p.V);
   KW8_REQUIRE(B * c < (1ll << 31), KW8_ERR_UNSUPPORTED, "too many rows");
@@ -948,7 +961,7 @@ int launch_typed(SampleArgs p, int64_t B, int64_t c, cudaStream_t stream) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  KW8_CUDA_TRY(cudaLaunchKernelEx(&cfg, sample_kernel<E, kThreads>, p));
+  KW8_CUDA_TRY(cudaLaunchKernelEx(&cfg, sample_kernel<E, kThreads, kStaged>, p));
   return KW8_OK;
 }
 
@@ -968,7 +981,14 @@ int launch_split(const SampleArgs& p, int64_t B, cudaStream_t stream) {
   const int64_t fit = std::min<int64_t>(
       65535, (kMaxSmem - 16 - static_cast<int64_t>(sizeof(SampShared))) / static_cast<int64_t>(sizeof(E)));
   while (c < 8 && c * fit < p.V) c *= 2;
-  return launch_typed<E, 512>(p, B, c, stream);
+  // Slices that leave room for one CTA per SM only, and more CTAs than SMs: read
+  // from L1 and L2 again, so that two CTAs share an SM (64 x 151936 fp32 top-k 50:
+  // 27 us, staged 35; top-p 0.9: 110 against 123).  Not where every token is
+  // weighed and nothing filtered (256 x 32000 fp32: 26 us, staged 24.5).
+  const bool filters = per_row || p.top_k0 > 0 || p.top_p0 < 1.f || p.min_p0 > 0.f;
+  const int64_t smem = static_cast<int64_t>(sizeof(SampShared)) + (p.V + c - 1) / c * static_cast<int64_t>(sizeof(E)) + 16;
+  if (smem > 113 * 1024 && c * B > 148 && filters) return launch_typed<E, 512, false>(p, B, c, stream);
+  return launch_typed<E, 512, true>(p, B, c, stream);
 }
 
 }  // namespace
