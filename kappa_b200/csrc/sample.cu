@@ -797,7 +797,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           },
           always);
       R.reduce3(lo, hi, count);
-      while (lo != hi) {
+      // Each level leaves 2^10 times fewer values: four at most.
+      for (int level = 0; level < 4 && lo != hi; ++level) {
         const int bits = 32 - __clz(static_cast<int>(hi - lo));
         const int shift = max(0, bits - 10);
         R.clear(by_mass);
@@ -805,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         for_each(
             [&](float v, int) {
               if (v >= least_v && v <= most_v) {
-                const int b = static_cast<int>((hi - order_key(v)) >> shift);
+                const int b = static_cast<int>((hi - order_key(v)) >> shift) & (kBins - 1);
                 atomicAdd(&sh.count[b], 1u);
                 if (by_mass) R.add_mass(b, weight(v));
               }

@@ -65,7 +65,7 @@ def test_packed_weights_give_the_same_bits(T, K, N):
         assert torch.equal(qlin.linear_q8(x, pack_weight(w, in_axis=-1), out_dtype=dtype), _ref(x, w, dtype))
 
 
-@pytest.mark.parametrize("T,K,N", [(300, 64, 1), (300, 64, 3), (257, 64, 63), (257, 64, 65), (270, 80, 127), (513, 64, 255), (258, 64, 258),
+@pytest.mark.parametrize("T,K,N", [(300, 64, 1), (300, 64, 3), (300, 64, 8), (260, 64, 16), (300, 64, 24), (257, 64, 72), (257, 64, 63), (257, 64, 65), (270, 80, 127), (513, 64, 255), (258, 64, 258),
                                    (400, 48, 301)])
 def test_widths_around_the_tiles(T, K, N):
     """Output rows that start at every alignment, ends inside a word, a box and a tile."""
