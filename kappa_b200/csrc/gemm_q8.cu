@@ -1,8 +1,6 @@
 // W8A8 linear: kernels and launcher (see gemm_q8.cuh).
 #include "gemm_q8.cuh"
 
-#include <cmath>
-
 #include "gemm_tc.cuh"
 #include "pack.cuh"
 
@@ -746,15 +744,18 @@ int launch_single(const int8_t* q, const kw8_weight& w, Q8LinearArgs p, int dev,
   // small; the weights' second and later reads come from L2 (77 x 2560 x 10243:
   // 32-row tiles 11.6 us, one 80-row tile 13 us).  64 where many rows meet a
   // deep K (128 x 9728 x 2560: 64 rows 13.9 us, 32 rows 14.6).
-  p.nt = static_cast<int>(std::min<int64_t>(T > kQ8PairRows ? 64 : 32, (T + 15) / 16 * 16));
+  // And where the tiles are many anyhow (64 x 2048 x 151936: 66 us, 32 rows 74).
+  const int64_t m_tiles = (N + kQ8Rows - 1) / kQ8Rows;
+  const bool many = m_tiles >= 4 * sms;
+  p.nt = static_cast<int>(std::min<int64_t>(many || T > kQ8PairRows ? 64 : 32, (T + 15) / 16 * 16));
   const int stage_bytes = kQ8ABytes + p.nt * kQ8BK;
-  const int64_t m_tiles = (N + kQ8Rows - 1) / kQ8Rows, t_tiles = (T + p.nt - 1) / p.nt;
+  const int64_t t_tiles = (T + p.nt - 1) / p.nt;
   // Ring: about 108 KB, two CTAs on an SM (16 x 2560 x 10240: three CTAs of 72
   // KB 10.1 us, two 9.4 us); 72 KB where CTAs follow one another and a third one
   // covers their starts and ends (16 x 2048 x 151936: 56 against 59 us).  Never
   // more CTAs on an SM than its 512 TMEM columns serve, so no allocation waits
   // for another CTA.
-  p.stages = std::min(kQ8MaxStages, (m_tiles * t_tiles >= 4 * sms ? 72 : 108) * 1024 / stage_bytes);
+  p.stages = std::min(kQ8MaxStages, (many ? 72 : 108) * 1024 / stage_bytes);
   const int smem_bytes = p.stages * stage_bytes + 1024;
   KW8_REQUIRE(p.stages >= 3 && smem_bytes >= q8_cols(p.nt) * 455 &&
                   p.nt * kQ8Rows * 4 <= p.stages * stage_bytes && smem_bytes <= kTcDynSmemMax,
@@ -767,10 +768,10 @@ int launch_single(const int8_t* q, const kw8_weight& w, Q8LinearArgs p, int dev,
   const double floor_us = static_cast<double>(N) * static_cast<double>(K) / 6e6;
   double best = 1e30;
   for (int ks = 1; ks <= 8; ++ks) {
-    if (valid_k_splits(ks, k_tiles) != ks) continue;
+    // More CTAs than are resident at once never pay for a split.
+    if (valid_k_splits(ks, k_tiles) != ks || (ks > 1 && tiles * ks > 2.0 * static_cast<double>(sms))) continue;
     const double per = static_cast<double>((k_tiles + ks - 1) / ks);
-    const double ctas = tiles * ks, resident = 2.0 * static_cast<double>(sms);
-    const double load = ctas <= resident ? std::max(1.0, 1.4 * ctas / resident) : 1.4 * std::ceil(ctas / resident);
+    const double load = std::max(1.0, 0.7 * tiles * ks / static_cast<double>(sms));
     const double us = std::max(floor_us, per * 0.25 * load) + (ks > 1 ? 0.9 + 0.1 * ks : 0.0);
     if (us < best) {
       best = us;
@@ -811,7 +812,9 @@ int launch_linear_q8(const int8_t* q, const kw8_weight& w, const Q8LinearArgs& a
   // meets few tiles, which only the other one splits (256 x 9728 x 2560: 17.4
   // against 16.6 us, 128 x 9728 x 2560: 17.6 against 13.9).
   const bool deep = p.T <= 256 && p.K >= 40 * kQ8BK && (p.N + 63) / 64 <= num_sms(dev) / 2;
-  const bool pair = p.T > kQ8PairRows && !deep;
+  // Many feature tiles: from 65 rows on (80 x 2048 x 151936: 71 us, else 74).
+  const bool many = p.T > 64 && (p.N + kQ8Rows - 1) / kQ8Rows >= 4 * num_sms(dev);
+  const bool pair = many || (p.T > kQ8PairRows && !deep);
   return pair ? launch_pair(q, w, p, dev, stream) : launch_single(q, w, p, dev, stream);
 }
 
