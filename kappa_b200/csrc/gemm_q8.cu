@@ -292,7 +292,6 @@ __global__ void __launch_bounds__(kQ8Threads)
 //               time, where the output's rows are no 16-byte multiples).
 
 constexpr int kQ8PairEpiWarps = 8;
-constexpr int kQ8PairRows = 96;  // more rows than this go to pairs
 constexpr int kQ8PairThreads = 128 + 32 * kQ8PairEpiWarps;
 constexpr int kQ8PairMaxStages = 8;
 constexpr int kQ8BoxBytes = 32 * 128;  // one warp's output box
@@ -662,6 +661,64 @@ int q8_cols(int nt) {
   return c;
 }
 
+// The choice between the two kernels, their tiles and the K splits is the least
+// of these models (us beyond a common part), fitted to 657 shapes of 17 to 1000
+// rows, K 64 to 9728 and 64 to 40960 channels: 1.8% above the best of the
+// measured choices on average, 31% at worst.  Both sides of it: 96 x 2048 x 4096
+// 8.4 us here, 7.3 with pairs; 77 x 2560 x 10243 11 us, 12.7 with pairs; 256 x 9728
+// x 64 8 us, 15 with pairs; 64 x 2048 x 151936 66 us with 64-row tiles, 74 with
+// 32-row ones, 69 with pairs.
+//
+// One CTA per tile of nt rows: a k tile takes 0.25 us and a tile 1.25 us more
+// (2.4 with 64 rows), shared by the CTAs of an SM; the weights come no faster
+// than 6 TB/s; joining ks parts of K costs 0.9 + 0.1 ks, and pays only while all
+// of them are resident (80 x 2048 x 151936 in 8 parts: 536 us, in one 74).
+double plan_single(Q8LinearArgs& p, int dev, int rows) {
+  const int64_t T = p.T, N = p.N, K = p.K, k_tiles = (K + kQ8BK - 1) / kQ8BK;
+  p.nt = static_cast<int>(std::min<int64_t>(rows, (T + 15) / 16 * 16));
+  const double tiles = static_cast<double>((N + kQ8Rows - 1) / kQ8Rows * ((T + p.nt - 1) / p.nt));
+  const double sms = num_sms(dev), weights = static_cast<double>(N) * static_cast<double>(K) / 6e6;
+  double best = 1e30, total = 0.0;
+  for (int ks = 1; ks <= 8; ++ks) {
+    if (valid_k_splits(ks, k_tiles) != ks || (ks > 1 && tiles * ks > 2 * sms)) continue;
+    const double k_us = static_cast<double>((k_tiles + ks - 1) / ks) * 0.25, tile_us = p.nt <= 32 ? 1.25 : 2.4;
+    const double load = std::max(1.0, 0.7 * tiles * ks / sms), join = ks > 1 ? 0.9 + 0.1 * ks : 0.0;
+    // The split that does the k tiles fastest (1 x 2048 x 4096: 4 parts 6.0 us, 6 parts 7.5, one 8).
+    const double us = std::max(weights, k_us * load) + join;
+    if (us < best) {
+      best = us;
+      p.k_splits = ks;
+      total = std::max(weights, (k_us + tile_us) * load) + join;
+    }
+  }
+  return total;
+}
+
+// Output rows that a TMA store can write.
+bool tma_rows(const Q8LinearArgs& p) {
+  return static_cast<int64_t>(p.N) * (p.out_f32 ? 4 : 2) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+}
+
+// Pairs: the channels per tile with the fewest waves, a wave costing its
+// channels plus a fixed part; a k tile takes 0.13 us at least, 0.29 at 256
+// channels; output rows that TMA cannot store 1.5 us more.
+double plan_pair(Q8LinearArgs& p, int dev) {
+  const int64_t T = p.T, N = p.N, K = p.K, pairs = num_sms(dev) / 2;
+  int64_t best = INT64_MAX, waves = 1;
+  for (int nt = 256; nt >= 64; nt -= 64) {
+    const int64_t w = ((T + 255) / 256 * ((N + nt - 1) / nt) + pairs - 1) / pairs;
+    if (w * (nt + 32) < best) {
+      best = w * (nt + 32);
+      waves = w;
+      p.nt = nt;
+    }
+  }
+  const double k_tile = std::max(0.13, 0.29 * p.nt / 256);
+  return std::max(static_cast<double>(N) * static_cast<double>(K) / 6e6,
+                  static_cast<double>(waves) * (static_cast<double>((K + kQ8BK - 1) / kQ8BK) * k_tile + 1.0)) +
+         (tma_rows(p) ? 1.0 : 2.5);
+}
+
 int make_w_map(CUtensorMap* map, const kw8_weight& w, int64_t N, int64_t K, int rows) {
   if (w.layout == KW8_LAYOUT_TILED)
     return make_tmap_tiled(map, w.q, static_cast<uint64_t>(tiled_ftiles(N)), static_cast<uint64_t>(tiled_steps(K)),
@@ -688,7 +745,7 @@ constexpr int kQ8PairSmem = 232448 - 9216;  // opt-in limit minus the static par
 
 int launch_pair(const int8_t* q, const kw8_weight& w, Q8LinearArgs p, int dev, cudaStream_t stream) {
   const int64_t esize = p.out_f32 ? 4 : 2;
-  const bool tma = p.N * esize % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+  const bool tma = tma_rows(p);
   const int kind = (p.out_f32 ? 2 : 0) + (tma ? 1 : 0);
   using Kernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const Q8PairArgs);
   static const Kernel kernels[4] = {linear_q8_pair_kernel<false, false>, linear_q8_pair_kernel<false, true>,
@@ -696,20 +753,9 @@ int launch_pair(const int8_t* q, const kw8_weight& w, Q8LinearArgs p, int dev, c
   static std::atomic<uint64_t> attr_set[4];
   int rc = allow_smem(kernels[kind], dev, attr_set[kind], kQ8PairSmem);
   if (rc) return rc;
-  const int64_t T = p.T, N = p.N, K = p.K;
-  const int64_t pairs = num_sms(dev) / 2;
+  const int64_t T = p.T, N = p.N, K = p.K, pairs = num_sms(dev) / 2;
   Q8PairArgs a{};
   a.t_tiles = static_cast<int>((T + 255) / 256);
-  // Channels per tile: the fewest waves over the SM pairs, a wave costing its channels plus a fixed part.
-  int64_t best = INT64_MAX;
-  for (int nt = 256; nt >= 64; nt -= 64) {
-    const int64_t tiles = a.t_tiles * ((N + nt - 1) / nt);
-    const int64_t cost = (tiles + pairs - 1) / pairs * (nt + 32);
-    if (cost < best) {
-      best = cost;
-      p.nt = nt;
-    }
-  }
   a.n_tiles = static_cast<int>((N + p.nt - 1) / p.nt);
   const int stage_bytes = kQ8ABytes + p.nt / 2 * kQ8BK;
   // A short K leaves the epilogue little time to hide in: two boxes per warp; a
@@ -739,45 +785,18 @@ int launch_single(const int8_t* q, const kw8_weight& w, Q8LinearArgs p, int dev,
   int rc = allow_smem(linear_q8_kernel, dev, attr_set, kTcDynSmemMax);
   if (rc) return rc;
   const int64_t T = p.T, N = p.N, K = p.K;
-  const int64_t sms = num_sms(dev), k_tiles = (K + kQ8BK - 1) / kQ8BK;
-  // Rows per tile: 32 at most, so that tiles are many and their exchanges
-  // small; the weights' second and later reads come from L2 (77 x 2560 x 10243:
-  // 32-row tiles 11.6 us, one 80-row tile 13 us).  64 where many rows meet a
-  // deep K (128 x 9728 x 2560: 64 rows 13.9 us, 32 rows 14.6).
-  // And where the tiles are many anyhow (64 x 2048 x 151936: 66 us, 32 rows 74).
-  const int64_t m_tiles = (N + kQ8Rows - 1) / kQ8Rows;
-  const bool many = m_tiles >= 4 * sms;
-  p.nt = static_cast<int>(std::min<int64_t>(many || T > kQ8PairRows ? 64 : 32, (T + 15) / 16 * 16));
+  const int64_t m_tiles = (N + kQ8Rows - 1) / kQ8Rows, t_tiles = (T + p.nt - 1) / p.nt;
   const int stage_bytes = kQ8ABytes + p.nt * kQ8BK;
-  const int64_t t_tiles = (T + p.nt - 1) / p.nt;
   // Ring: about 108 KB, two CTAs on an SM (16 x 2560 x 10240: three CTAs of 72
   // KB 10.1 us, two 9.4 us); 72 KB where CTAs follow one another and a third one
   // covers their starts and ends (16 x 2048 x 151936: 56 against 59 us).  Never
   // more CTAs on an SM than its 512 TMEM columns serve, so no allocation waits
   // for another CTA.
-  p.stages = std::min(kQ8MaxStages, (many ? 72 : 108) * 1024 / stage_bytes);
+  p.stages = std::min(kQ8MaxStages, (m_tiles >= 4 * num_sms(dev) ? 72 : 108) * 1024 / stage_bytes);
   const int smem_bytes = p.stages * stage_bytes + 1024;
   KW8_REQUIRE(p.stages >= 3 && smem_bytes >= q8_cols(p.nt) * 455 &&
                   p.nt * kQ8Rows * 4 <= p.stages * stage_bytes && smem_bytes <= kTcDynSmemMax,
               KW8_ERR_UNSUPPORTED, "no pipeline plan for %d-row tiles", p.nt);
-  // K splits: the least of a model in us that the measured sweeps gave: a k
-  // tile takes about 0.25 us per CTA (shared by the CTAs of an SM), the weights
-  // cannot come faster than 6 TB/s, and joining the sums costs 0.9 + 0.1 per
-  // part (1 x 2048 x 4096: 4 parts 6.0 us, 1 part 8, 8 parts 7.4).
-  const double tiles = static_cast<double>(m_tiles * t_tiles);
-  const double floor_us = static_cast<double>(N) * static_cast<double>(K) / 6e6;
-  double best = 1e30;
-  for (int ks = 1; ks <= 8; ++ks) {
-    // More CTAs than are resident at once never pay for a split.
-    if (valid_k_splits(ks, k_tiles) != ks || (ks > 1 && tiles * ks > 2.0 * static_cast<double>(sms))) continue;
-    const double per = static_cast<double>((k_tiles + ks - 1) / ks);
-    const double load = std::max(1.0, 0.7 * tiles * ks / static_cast<double>(sms));
-    const double us = std::max(floor_us, per * 0.25 * load) + (ks > 1 ? 0.9 + 0.1 * ks : 0.0);
-    if (us < best) {
-      best = us;
-      p.k_splits = ks;
-    }
-  }
   CUtensorMap map_w, map_x;
   rc = make_w_map(&map_w, w, N, K, kQ8Rows);
   if (!rc) rc = make_x_map(&map_x, q, T, K, p.nt);
@@ -807,15 +826,11 @@ int launch_linear_q8(const int8_t* q, const kw8_weight& w, const Q8LinearArgs& a
   p.w_scale_pc = w.per_channel;
   int dev = 0;
   KW8_CUDA_TRY(cudaGetDevice(&dev));
-  // Above kQ8PairRows rows the pair kernel is faster (128 x 2048 x 4096: 7.4 us
-  // against 8.2; 100 rows or fewer the other way round), but not where a deep K
-  // meets few tiles, which only the other one splits (256 x 9728 x 2560: 17.4
-  // against 16.6 us, 128 x 9728 x 2560: 17.6 against 13.9).
-  const bool deep = p.T <= 256 && p.K >= 40 * kQ8BK && (p.N + 63) / 64 <= num_sms(dev) / 2;
-  // Many feature tiles: from 65 rows on (80 x 2048 x 151936: 71 us, else 74).
-  const bool many = p.T > 64 && (p.N + kQ8Rows - 1) / kQ8Rows >= 4 * num_sms(dev);
-  const bool pair = many || (p.T > kQ8PairRows && !deep);
-  return pair ? launch_pair(q, w, p, dev, stream) : launch_single(q, w, p, dev, stream);
+  Q8LinearArgs narrow = p, wide = p, pair = p;
+  const double narrow_us = plan_single(narrow, dev, 32), wide_us = p.T > 32 ? plan_single(wide, dev, 64) : 1e30;
+  const double pair_us = p.T > 32 ? plan_pair(pair, dev) : 1e30, single_us = std::min(narrow_us, wide_us);
+  if (pair_us < single_us) return launch_pair(q, w, pair, dev, stream);
+  return launch_single(q, w, wide_us < narrow_us ? wide : narrow, dev, stream);
 }
 
 }  // namespace kw8

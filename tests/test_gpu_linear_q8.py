@@ -58,7 +58,19 @@ def test_linear_q8(T, K, N, dtype):
         assert y.dtype == dtype and torch.equal(y, _ref(x, w, dtype))
 
 
-@pytest.mark.parametrize("T,K,N", [(1, 208, 100), (16, 2048, 512), (50, 1040, 257), (256, 512, 256), (300, 2048, 1030), (700, 272, 2000)])
+@pytest.mark.parametrize("T,K,N", [(1100, 64, 1000), (1100, 272, 1021), (1100, 2064, 1025), (2049, 64, 1024), (2049, 272, 511),
+                                   (2049, 2576, 1090), (4100, 144, 2049), (4100, 2048, 640),
+                                   (257, 9728, 10240), (300, 9728, 10243), (513, 5136, 20480)])
+def test_many_rows(T, K, N):
+    """Sizes that go to the pair kernel: several tiles a pair, ends inside them, one and two output boxes a warp, a few rows
+    behind the last whole tile."""
+    x, w = _rows(T, K, N), _weight(N, K, T)
+    for dtype in (torch.bfloat16, torch.float32):
+        assert torch.equal(qlin.linear_q8(x, w, out_dtype=dtype), _ref(x, w, dtype))
+
+
+@pytest.mark.parametrize("T,K,N", [(1, 208, 100), (16, 2048, 512), (50, 1040, 257), (256, 512, 256), (300, 2048, 1030), (700, 272, 2000),
+                                   (2049, 272, 1030), (30000, 64, 48)])
 def test_packed_weights_give_the_same_bits(T, K, N):
     x, w = _rows(T, K, 5), _weight(N, K, 6)
     for dtype in (torch.bfloat16, torch.float32):
@@ -66,7 +78,8 @@ def test_packed_weights_give_the_same_bits(T, K, N):
 
 
 @pytest.mark.parametrize("T,K,N", [(300, 64, 1), (300, 64, 3), (300, 64, 8), (260, 64, 16), (300, 64, 24), (257, 64, 72), (257, 64, 63), (257, 64, 65), (270, 80, 127), (513, 64, 255), (258, 64, 258),
-                                   (400, 48, 301)])
+                                   (400, 48, 301)]
+                         + [(30000, 64, N) for N in (1, 2, 3, 7, 8, 15, 16, 17, 63, 64, 65, 66)])
 def test_widths_around_the_tiles(T, K, N):
     """Output rows that start at every alignment, ends inside a word, a box and a tile."""
     x, w = _rows(T, K, N), _weight(N, K, N)
@@ -86,7 +99,7 @@ def test_widths_around_the_tiles(T, K, N):
 def test_largest_sums():
     """Every product at its extreme: the sum reaches 128 * 128 * K just below 2^31."""
     K = 131056
-    for T, N in ((3, 20), (300, 300)):
+    for T, N in ((3, 20), (300, 300), (1000, 1000)):
         for a, b in ((-128, -128), (-128, 127), (127, 127)):
             x = Q8Rows(torch.full((T, K), a, dtype=torch.int8, device="cuda"), torch.ones(T, 1, device="cuda"))
             w = Q8Weight(torch.full((N, K), b, dtype=torch.int8, device="cuda"), torch.ones(N, 1, device="cuda"))
@@ -148,7 +161,7 @@ def test_projections_and_head_take_8_bit_rows():
 def test_rows_behind_the_last_are_left_alone():
     """The kernel writes T rows of N values and nothing else."""
     lib = _lib.load()
-    for T, K, N in ((3, 256, 100), (130, 256, 136), (300, 256, 520)):
+    for T, K, N in ((3, 256, 100), (130, 256, 136), (300, 256, 520), (2100, 256, 1036), (2100, 256, 1037)):
         x, w = _rows(T, K, 1), _weight(N, K, 2)
         out = torch.full((T + 8, N), 7.0, dtype=torch.bfloat16, device="cuda")
         wk = _lib.KW8Weight(w.values.data_ptr(), w.scale.data_ptr(), _lib.DT_F32, 1, 0, 0)
