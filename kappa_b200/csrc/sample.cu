@@ -21,7 +21,10 @@
 //   M <= kList: one CTA collects, sorts and finishes them (the usual settings);
 //   else (flat rows, many ties, a wide nucleus): the cut is narrowed inside its
 //   bin by histograms over the ordered bit patterns until one value is left,
-//   whose ties are kept by index, and every CTA draws from its slice.
+//   whose ties are kept by index, and every CTA draws from its slice.  For top-p
+//   alone the pass that sums the weights also lists the tokens of the bins that
+//   the cut can lie in, and those steps go through them alone (64 x 151936 fp32,
+//   top-p 0.9: 72 us, 110 through all tokens).
 // CTAs add their histograms through distributed shared memory.
 #include "sample.cuh"
 
@@ -32,8 +35,10 @@ namespace kw8 {
 namespace {
 
 constexpr int kBins = 1024;
+constexpr int kBinParts = 1024;    // positions told apart inside a bin where a top-p cut is bounded
 constexpr float kBinSpan = 32.f;  // e-folds of the weight over all bins: the last one holds weights of 0
 constexpr int kList = 1024;       // tokens that one CTA sorts
+constexpr int kWindow = 2048;     // tokens around a top-p cut that a CTA lists
 constexpr int kRanked = 256;      // up to here by counting, above by a sorting network
 constexpr int kMaxRanks = 16;
 constexpr int kMaxSmem = 232448;
@@ -93,11 +98,6 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ u64 ld_cluster_u64(uint32_t addr) {
-  u64 v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
-  return v;
-}
 __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
@@ -126,17 +126,32 @@ struct alignas(16) SampShared {
   };
   double exp_table[kExpSteps * kExpCopies];  // 2^(44 - i / kExpSteps)
   u64 warp_a[32];
-  u64 pub[2][kMaxRanks][3];  // every CTA's values of a cluster-wide reduction (alternating)
+  u64 warp_all[16][4];
+  u64 pub[2][kMaxRanks][4];  // every CTA's values of a cluster-wide reduction (alternating)
   u64 cut_before;            // sum in front of the cut's bin
   uint32_t cut_bin, cut_count;
   uint32_t first_bin;           // of a top-p cut's window
+  uint32_t windowed;            // its tokens in this CTA (entries of `window` while they fit)
+  uint16_t window[kWindow];
   uint32_t listed;              // tokens of this CTA down to the cut (entries of `list` while they fit)
   uint32_t lists[kMaxRanks];    // every CTA's
 };
 
+__device__ __forceinline__ u64 max64(u64 a, u64 b) { return a > b ? a : b; }
+__device__ __forceinline__ u64 min64(u64 a, u64 b) { return a < b ? a : b; }
+__device__ __forceinline__ u64 add64(u64 a, u64 b) { return a + b; }
+
+// The least and the largest of some order keys, 0 for none, and two of these joined.
+__device__ __forceinline__ u64 range(uint32_t lo, uint32_t hi) { return (static_cast<u64>(hi) << 32) | (~lo & 0xffffffffu); }
+__device__ __forceinline__ u64 wider(u64 a, u64 b) {
+  return (static_cast<u64>(max(static_cast<uint32_t>(a >> 32), static_cast<uint32_t>(b >> 32))) << 32) |
+         max(static_cast<uint32_t>(a), static_cast<uint32_t>(b));
+}
+
 template <int kThreads>
 struct Row {
   static constexpr int kWarps = kThreads / 32;
+  static_assert(kWarps <= 16);
   SampShared& sh;
   const int ranks, rank;
   int turn = 0;
@@ -167,13 +182,13 @@ struct Row {
   // Stores this CTA's values into every CTA's slot for it (thread r into CTA
   // r), and waits for all of them.  The slots alternate, so the last ones may
   // still be read meanwhile.
-  __device__ __forceinline__ void publish(u64 a, u64 b, u64 c) {
+  template <int kN>
+  __device__ __forceinline__ void publish(const u64 (&v)[kN]) {
     turn ^= 1;
     if (static_cast<int>(threadIdx.x) < ranks) {
       const uint32_t at = mapa_shared(smem_u32(sh.pub[turn][rank]), threadIdx.x);
-      st_cluster_u64(at, a);
-      st_cluster_u64(at + 8, b);
-      st_cluster_u64(at + 16, c);
+#pragma unroll
+      for (int j = 0; j < kN; ++j) st_cluster_u64(at + 8 * j, v[j]);
     }
     cluster_sync_all();
   }
@@ -183,27 +198,40 @@ struct Row {
   __device__ __forceinline__ u64 reduce(u64 v, Op op) {
     v = block_reduce(v, op);
     if (ranks == 1) return v;
-    publish(v, 0, 0);
+    publish({v});
     u64 r = sh.pub[turn][0][0];
     for (int i = 1; i < ranks; ++i) r = op(r, sh.pub[turn][i][0]);
     return r;
   }
 
-  // The same for a least value, a largest one and a sum at once.
-  __device__ __forceinline__ void reduce3(u64& lo, u64& hi, u64& sum) {
-    const auto mn = [](u64 a, u64 b) { return a < b ? a : b; };
-    const auto mx = [](u64 a, u64 b) { return a > b ? a : b; };
-    lo = block_reduce(lo, mn);
-    hi = block_reduce(hi, mx);
-    sum = block_reduce(sum, [](u64 a, u64 b) { return a + b; });
-    if (ranks == 1) return;
-    publish(lo, hi, sum);
-    sum = 0;
-    for (int i = 0; i < ranks; ++i) {
-      lo = mn(lo, sh.pub[turn][i][0]);
-      hi = mx(hi, sh.pub[turn][i][1]);
-      sum += sh.pub[turn][i][2];
+  // The same for a few sums and one range() at once.
+  __device__ __forceinline__ void reduce_all(u64 (&v)[4]) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+      for (int j = 0; j < 3; ++j) v[j] += __shfl_xor_sync(0xffffffffu, v[j], o);
+      v[3] = wider(v[3], __shfl_xor_sync(0xffffffffu, v[3], o));
     }
+    const int slot = threadIdx.x >> 5;
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sh.warp_all[slot][j] = v[j];
+    }
+    __syncthreads();
+    const auto add_up = [&](const auto& all, int n) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = all[0][j];
+      for (int i = 1; i < n; ++i) {
+#pragma unroll
+        for (int j = 0; j < 3; ++j) v[j] += all[i][j];
+        v[3] = wider(v[3], all[i][3]);
+      }
+    };
+    add_up(sh.warp_all, kWarps);
+    if (ranks == 1) return;
+    publish(v);
+    add_up(sh.pub[turn], ranks);
   }
 
   // Exclusive prefix of v over this CTA's threads; `all` is their sum.
@@ -235,7 +263,7 @@ struct Row {
     u64 at = block_prefix(v, all);
     total = all;
     if (ranks > 1) {
-      publish(all, 0, 0);
+      publish({all});
       total = 0;
       for (int i = 0; i < ranks; ++i) {
         const u64 c = sh.pub[turn][i][0];
@@ -264,8 +292,9 @@ struct Row {
   }
 
   // Adds the CTAs' histograms: each sums its share of the bins, some threads
-  // to a bin, and stores it into every CTA's copy.
-  __device__ __forceinline__ void sum(bool count, bool mass) {
+  // to a bin, and stores it into every CTA's copy.  Of the masses all three
+  // pieces, or the first alone.
+  __device__ __forceinline__ void sum(bool count, bool mass, bool pieces = true) {
     sync();
     const int share = (kBins + ranks - 1) / ranks;
     const int group = ranks >= 4 && kThreads >= 4 * share ? 4 : ranks >= 2 && kThreads >= 2 * share ? 2 : 1;
@@ -281,9 +310,9 @@ struct Row {
         for (int i = part; i < ranks; i += group) {
           const uint32_t r = static_cast<uint32_t>(i);
           if (count) c += ld_cluster_u32(mapa_shared(smem_u32(&sh.count[b]), r));
-          if (mass)
-            m += ld_cluster_u32(mapa_shared(smem_u32(&sh.mass[0][b]), r)) +
-                 (static_cast<u64>(ld_cluster_u32(mapa_shared(smem_u32(&sh.mass[1][b]), r))) << 16) +
+          if (mass) m += ld_cluster_u32(mapa_shared(smem_u32(&sh.mass[0][b]), r));
+          if (mass && pieces)
+            m += (static_cast<u64>(ld_cluster_u32(mapa_shared(smem_u32(&sh.mass[1][b]), r))) << 16) +
                  (static_cast<u64>(ld_cluster_u32(mapa_shared(smem_u32(&sh.mass[2][b]), r))) << 32);
         }
       for (int o = 1; o < group; o <<= 1) {
@@ -328,21 +357,31 @@ struct Row {
     __syncthreads();
   }
 
-  // From the counts alone: the bins between which the top_p cut must lie.  The
-  // weights of bin b are in 2^44 e^(-(b + 1.02) s) - 1 .. 2^44 e^(-(b - 0.02) s), s the
-  // bins' span (0.02: the roundings of the bin).  sh.first_bin: the first that it
-  // can lie in, sh.cut_bin: the first that it cannot lie behind (as it was, where
-  // the bounds do not tell).
-  __device__ __forceinline__ void bound_cut(double top_p) {
+  // From the counts, and where `fine` from the positions inside the bins
+  // (count_positions()): the bins between which the top_p cut must lie.  The
+  // exponential is convex: with s the bins' span, the weights of bin b's c tokens,
+  // whose positions in it have the sum S, add up to at most e^(-b s) (c - S (1 - e^-s))
+  // (the chord) and to at least e^(-(b + 1/2) s) (c - (S - c / 2) s) (the tangent in
+  // the middle), 0.024% less; without S 3% lie between its ends.  Besides, positions
+  // are rounded down to 2^-10 bins and weights to whole numbers, and 3 roundings of
+  // 2^-24 move a position by at most 0.0002 bins.  sh.first_bin: the first bin that
+  // the cut can lie in, sh.cut_bin: the first that it cannot lie behind (as it was,
+  // where the bounds do not tell).
+  __device__ __forceinline__ void bound_cut(double top_p, bool fine) {
     constexpr int kPer = kBins / kThreads;
-    constexpr double kSpan = static_cast<double>(kBinSpan) / (kBins - 1);
+    constexpr double kSpan = static_cast<double>(kBinSpan) / (kBins - 1), kMoved = 0.0005;
+    constexpr double kStep = kSpan * (1 - kSpan / 2);                          // at most 1 - e^-s
+    constexpr double kHalf = 1 - kSpan / 2 * (1 - kSpan / 4 * (1 - kSpan / 6));  // at most e^(-s / 2)
     u64 lo[kPer], hi[kPer], slo = 0, shi = 0, all_lo, all_hi;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int b = threadIdx.x * kPer + j;
-      const double w = kOne * exp(-(b + 1.02) * kSpan);
-      lo[j] = sh.count_sum[b] * static_cast<u64>(fmax(floor(w) - 1.0, 0.0));
-      hi[j] = sh.count_sum[b] * static_cast<u64>(ceil(w * 1.0336));  // e^(1.04 s) = 1.03307
+      const double c = sh.count_sum[b], S = fine ? static_cast<double>(sh.mass_sum[b]) * (1.0 / kBinParts) : 0.0;
+      const double w = kOne * exp(-(b - kMoved) * kSpan);
+      const double most = c - S * kStep;
+      const double least = kHalf * (c - ((fine ? S + c * (1.0 / kBinParts) : c) + c * (2 * kMoved - 0.5)) * kSpan);
+      lo[j] = static_cast<u64>(fmax(w * least * (1 - 1e-12) - c, 0.0));
+      hi[j] = static_cast<u64>(ceil(w * most * (1 + 1e-12)));
       slo += lo[j];
       shi += hi[j];
     }
@@ -382,10 +421,6 @@ struct Row {
       }
   }
 };
-
-__device__ __forceinline__ u64 max64(u64 a, u64 b) { return a > b ? a : b; }
-__device__ __forceinline__ u64 min64(u64 a, u64 b) { return a < b ? a : b; }
-__device__ __forceinline__ u64 add64(u64 a, u64 b) { return a + b; }
 
 template <class E, int kThreads, bool kStaged>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -507,6 +542,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   // Monotone in v: a subtraction, a product cut to [0, 1], a product rounded
   // down (by adding 2^23).
   const float bin_scale = fminf(1.f / (kBinSpan * temp), 1e30f);
+  const bool linear = temp > 1e-31f;  // below, the last bin's weights need not be 0
   const auto bin_of = [&](float v) -> int {
     const float d = __saturatef((top - v) * bin_scale);
     return static_cast<int>(__float_as_uint(__fmaf_rz(d, static_cast<float>(kBins - 1), 8388608.f)) & (kBins - 1));
@@ -530,12 +566,23 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int i0 = min(n, tid * run_len), i1 = min(n, i0 + run_len);
   const auto over_run = [&](auto&& f) {
 #pragma unroll 4
-    for (int i = i0; i < i1; ++i) f(elem(i));
+    for (int i = i0; i < i1; ++i) f(elem(i), i);
   };
   // Sum of this thread's tokens above run_top, in front of the window in which a
   // mass cut lies: certain to stay, and summed already.
   u64 run_sum = 0;
   float run_top = INFINITY;
+
+  // Whether sh.window lists that window's tokens, and every one of the cluster's
+  // CTAs had room for its own.
+  bool listed = false;
+  u64 window_front = 0, window_count = 0, window_range = 0;  // the sum in front of it, its tokens, their keys
+
+  // The key of a cut: a bf16 number's upper half is enough.
+  const auto cut_key_of = [](float v) { return sizeof(E) == 2 ? order_key(v) >> 16 : order_key(v); };
+  const auto cut_value = [](uint32_t key) {
+    return key_value(sizeof(E) == 2 ? (key << 16) | (key & 0x8000u ? 0u : 0xFFFFu) : key);
+  };
 
   // The cut of the general path: tokens above cut_key stay, of those at it the first cut_ties.
   uint32_t cut_key = 0;
@@ -563,13 +610,34 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   };
   const auto always = [] { return true; };
+  // The same for the tokens that a cut can lie at.
+  const auto for_window = [&](auto&& f) {
+    if (listed) {
+      for (int i = tid; i < static_cast<int>(sh.windowed); i += kThreads) f(elem(sh.window[i]), sh.window[i]);
+    } else {
+      for_each(f, always);
+    }
+  };
   const auto count_all = [&] {
     for_each([&](float v, int) { atomicAdd(&sh.count[bin_of(v)], 1u); }, always);
   };
+  // And the sums of the positions inside the bins, in mass[0] (under 2^16 tokens of
+  // 10 bits).  The bin is bin_of's: both round the same product down.
+  const auto count_positions = [&] {
+    for_each(
+        [&](float v, int) {
+          const float d = __saturatef((top - v) * bin_scale);
+          const uint32_t at = __float_as_uint(__fmaf_rz(d, static_cast<float>((kBins - 1) * kBinParts), 8388608.f)) & (kBins * kBinParts - 1);
+          atomicAdd(&sh.count[at / kBinParts], 1u);
+          atomicAdd(&sh.mass[0][at / kBinParts], at % kBinParts);
+        },
+        always);
+  };
   if (use_k || use_p || use_m) {
-    const bool mass = use_p && !use_k;
-    // Counts find the bin of a top-k cut, and bound a top-p cut: a bin's weights
-    // differ by 3%, so the cut lies in a window of a few bins.
+    // Counts find the bin of a top-k cut, and bound a top-p cut, with the positions
+    // inside the bins to a window of a bin or two (not worth their sums where min_p
+    // bounds it besides: 16 x 262144 bf16, top-p 0.9, min-p 0.02: 37 us, 44 with them).
+    const bool mass = use_p && !use_k, fine = mass && !use_m;
     // When at least top_k threads hold a token, the top_k-th largest of the
     // threads' own largest logits already bounds the cut (that many tokens are
     // not below it), at one addition per thread instead of one per token.
@@ -577,20 +645,22 @@ __global__ void __launch_bounds__(kThreads, 2)
     double thr = 0.0;
     const bool by_threads = use_k && k <= kThreads * ranks / 2 && p.V >= kThreads * ranks;
     if (use_k || use_p) {
-      R.clear(false);
-      if (!by_threads)
+      R.clear(fine);
+      if (fine)
+        count_positions();
+      else if (!by_threads)
         count_all();
       else if (best_at >= 0)
         atomicAdd(&sh.count[bin_of(best)], 1u);
-      R.sum(true, false);
+      R.sum(true, fine, false);
       // Fewer threads than top_k above -inf: no bound, every token may be kept.
       sh.cut_bin = kBins - 1;
       sh.first_bin = 0;
       __syncthreads();
       if (use_k) {
         R.find_cut(false, static_cast<u64>(k), 0.0, 0);
-      } else if (temp > 1e-31f) {  // below, the bins are not linear in the logarithm
-        R.bound_cut(static_cast<double>(top_p));
+      } else if (linear) {
+        R.bound_cut(static_cast<double>(top_p), fine);
         if (sh.first_bin > 0) run_top = upper(static_cast<float>(sh.first_bin) - 0.5f);
       }
       last = static_cast<int>(sh.cut_bin);
@@ -604,30 +674,56 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (mass) {
       // All weights once: their sum, and where the list will not do (it reaches up
       // to two bins further, see below) this thread's part of it in front of the
-      // window, and the window's own histogram.
+      // window, and the tokens of the window, if there is room for them.
+      if (tid == 0) sh.windowed = 0;
       window = R.count_to(min(last + 2, kBins - 1)) > kList;
       u64 sum = 0;
       if (!window) {
-        over_run([&](float v) { sum += weight(v); });
+        over_run([&](float v, int) { sum += weight(v); });
+        sum = R.reduce(sum, add64);
       } else {
-        R.clear(true);
         const int window_end = static_cast<int>(sh.cut_bin);
-        const float window_low = lower(static_cast<float>(window_end) + 1.5f);
-        over_run([&](float v) {
+        const float window_low = linear ? lower(static_cast<float>(window_end) + 1.5f) : -INFINITY;
+        uint32_t lo = 0xffffffffu, hi = 0;
+        over_run([&](float v, int i) {
           const u64 w = weight(v);
           sum += w;
           run_sum += v > run_top ? w : 0;
           if (v <= run_top && v >= window_low) {
-            const int b = bin_of(v);
-            if (b <= window_end) R.add_mass(b, w);
+            const uint32_t at = atomicAdd(&sh.windowed, 1u);
+            if (at < kWindow) sh.window[at] = static_cast<uint16_t>(i);
           }
         });
+        __syncthreads();
+        for (int i = tid; i < min(static_cast<int>(sh.windowed), kWindow); i += kThreads) {
+          const uint32_t key = cut_key_of(elem(sh.window[i]));
+          lo = min(lo, key);
+          hi = max(hi, key);
+        }
+        const u64 room = sh.windowed <= kWindow ? 0 : 1ull << 32;
+        u64 all[4] = {sum, run_sum, tid == 0 ? sh.windowed + room : 0, range(lo, hi)};
+        R.reduce_all(all);
+        sum = all[0];
+        thr = static_cast<double>(top_p) * static_cast<double>(sum);
+        window_front = all[1];
+        window_count = all[2];
+        window_range = all[3];
+        listed = window_count < (1ull << 32);
+        if (!listed) {  // the bin of the cut first
+          R.clear(true);
+          for_each(
+              [&](float v, int) {
+                if (v <= run_top && v >= window_low) {
+                  const int b = bin_of(v);
+                  if (b <= window_end) R.add_mass(b, weight(v));
+                }
+              },
+              always);
+          R.sum(false, true);
+          R.find_cut(true, 0, thr, window_front);
+        }
       }
-      thr = static_cast<double>(top_p) * static_cast<double>(R.reduce(sum, add64));
-      if (window) {
-        R.sum(false, true);
-        R.find_cut(true, 0, thr, R.reduce(run_sum, add64));
-      }
+      thr = static_cast<double>(top_p) * static_cast<double>(sum);
     }
 
     // Collect the tokens down to bin `last` as (key, ~index), as far as they fit.
@@ -782,36 +878,41 @@ __global__ void __launch_bounds__(kThreads, 2)
     // The general path.  Inside the bin that sh's cut is in: the cut's key, its ties and how many of them stay.
     u64 ties_w = 0;
     const auto refine = [&](bool by_mass, u64 goal_k, double goal_p) {
-      u64 before = sh.cut_before;
-      const int bin = static_cast<int>(sh.cut_bin);
-      u64 lo = 0xffffffffu, hi = 0, count = 0;
-      const float above = bin > 0 ? upper(static_cast<float>(bin) - 0.5f) : INFINITY, below = lower(static_cast<float>(bin) + 1.5f);
-      for_each(
-          [&](float v, int) {
-            if (v <= above && v >= below && bin_of(v) == bin) {
-              const uint32_t key = order_key(v);
-              lo = min64(lo, key);
-              hi = max64(hi, key);
-              ++count;
-            }
-          },
-          always);
-      R.reduce3(lo, hi, count);
+      u64 before = window_front, count = window_count, keys = window_range;
+      if (!listed) {
+        before = sh.cut_before;
+        const int bin = static_cast<int>(sh.cut_bin);
+        const float above = bin > 0 ? upper(static_cast<float>(bin) - 0.5f) : INFINITY;
+        const float below = bin < kBins - 1 ? lower(static_cast<float>(bin) + 1.5f) : -INFINITY;
+        uint32_t lo = 0xffffffffu, hi = 0, mine = 0;
+        for_each(
+            [&](float v, int) {
+              if (v <= above && v >= below && bin_of(v) == bin) {
+                lo = min(lo, cut_key_of(v));
+                hi = max(hi, cut_key_of(v));
+                ++mine;
+              }
+            },
+            always);
+        u64 all[4] = {mine, 0, 0, range(lo, hi)};
+        R.reduce_all(all);
+        count = all[0];
+        keys = all[3];
+      }
+      u64 lo = ~static_cast<uint32_t>(keys), hi = keys >> 32;
       // Each level leaves 2^10 times fewer values: four at most.
       for (int level = 0; level < 4 && lo != hi; ++level) {
         const int bits = 32 - __clz(static_cast<int>(hi - lo));
         const int shift = max(0, bits - 10);
         R.clear(by_mass);
-        const float least_v = key_value(static_cast<uint32_t>(lo)), most_v = key_value(static_cast<uint32_t>(hi));
-        for_each(
-            [&](float v, int) {
-              if (v >= least_v && v <= most_v) {
-                const int b = static_cast<int>((hi - order_key(v)) >> shift) & (kBins - 1);
-                atomicAdd(&sh.count[b], 1u);
-                if (by_mass) R.add_mass(b, weight(v));
-              }
-            },
-            always);
+        const float least_v = cut_value(static_cast<uint32_t>(lo)), most_v = cut_value(static_cast<uint32_t>(hi));
+        for_window([&](float v, int) {
+          if (v >= least_v && v <= most_v) {
+            const int b = static_cast<int>((hi - cut_key_of(v)) >> shift) & (kBins - 1);
+            atomicAdd(&sh.count[b], 1u);
+            if (by_mass) R.add_mass(b, weight(v));
+          }
+        });
         R.sum(true, by_mass);
         R.find_cut(by_mass, goal_k, goal_p, before);
         before = sh.cut_before;
@@ -822,7 +923,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       // One value left.
       const uint32_t key = static_cast<uint32_t>(lo);
-      const u64 w = weight(key_value(key));
+      const u64 w = weight(cut_value(key));
       uint32_t ties;
       if (by_mass) {
         uint32_t a = 1, b = static_cast<uint32_t>(count);  // the first always stays: `before` is below the goal
@@ -850,11 +951,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       R.find_cut(false, static_cast<u64>(k), 0.0, 0);
     }
     // In the last bin every weight is 0: whatever is kept of it is never drawn.
-    if ((use_k || use_p) && sh.cut_bin < kBins - 1) refine(mass, static_cast<u64>(k), thr);
+    if (listed || ((use_k || use_p) && (sh.cut_bin < kBins - 1 || !linear))) refine(mass, static_cast<u64>(k), thr);
     if (use_k && use_p) {
       R.clear(true);
       u64 s = 0;
-      const float cut_v = cut_key == 0 ? -INFINITY : key_value(cut_key);
+      const float cut_v = cut_key == 0 ? -INFINITY : cut_value(cut_key);
       for_each(
           [&](float v, int) {
             if (v >= cut_v) {
@@ -874,20 +975,41 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 
   // The draw.
-  u64 rank_of_tie = 0;
-  if (cut_ties < cut_all) {
+  u64 rank_of_tie = 0, run_ties = 0;
+  const bool from_list = listed && !use_m;
+  if (from_list) {
+    // What stays of the window, by the thread in whose run it is.
+    const float cut_v = cut_key == 0 ? -INFINITY : cut_value(cut_key);
+    R.clear(true);
+    for_window([&](float v, int i) {
+      if (v > cut_v)
+        R.add_mass(i / run_len, weight(v));
+      else if (v == cut_v)
+        atomicAdd(&sh.count[i / run_len], 1u);
+    });
+    __syncthreads();
+    run_ties = sh.count[tid];
+    if (cut_ties < cut_all) {
+      u64 all;
+      rank_of_tie = R.prefix(run_ties, all);
+    }
+  } else if (cut_ties < cut_all) {
     u64 ties = 0, all;
-    const float cut_v = key_value(cut_key);
+    const float cut_v = cut_value(cut_key);
     for (int i = i0; i < i1; ++i) ties += elem(i) == cut_v;
     rank_of_tie = R.prefix(ties, all);
   }
   u64 mine = 0, total;
-  if (cut_key == 0 && !use_m) {
-    over_run([&](float v) { mine += weight(v); });
+  if (from_list) {
+    const u64 left = rank_of_tie < cut_ties ? cut_ties - rank_of_tie : 0;
+    mine = run_sum + sh.mass[0][tid] + (static_cast<u64>(sh.mass[1][tid]) << 16) + (static_cast<u64>(sh.mass[2][tid]) << 32);
+    if (cut_key != 0) mine += min64(run_ties, left) * weight(cut_value(cut_key));
+  } else if (cut_key == 0 && !use_m) {
+    over_run([&](float v, int) { mine += weight(v); });
   } else {
     // What is summed already is not evaluated again (min_p may cut in front of the window).
     const bool summed = run_top < INFINITY && !use_m;
-    const float cut_v = cut_key == 0 ? -INFINITY : key_value(cut_key);
+    const float cut_v = cut_key == 0 ? -INFINITY : cut_value(cut_key);
     if (summed) mine = run_sum;
     u64 tie = rank_of_tie;
     for (int i = i0; i < i1; ++i) {
@@ -908,7 +1030,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     u64 base = __shfl_sync(0xffffffffu, at, o), tie = __shfl_sync(0xffffffffu, rank_of_tie, o);
     for (int i = w0; i < w1; i += 32) {
       const float v = i + lane < w1 ? elem(i + lane) : -INFINITY;
-      const uint32_t key = order_key(v);
+      const uint32_t key = cut_key_of(v);
       const uint32_t ties = __ballot_sync(0xffffffffu, i + lane < w1 && key == cut_key);
       const bool out = i + lane >= w1 || key < cut_key ||
                        (key == cut_key && tie + __popc(ties & ((1u << lane) - 1)) >= cut_ties);
@@ -972,7 +1094,7 @@ int launch_typed(SampleArgs p, int64_t B, int64_t c, cudaStream_t stream) {
 // costs more in exchanges than it gains (256 x 32000 bf16: 1 CTA a row 20 us, 2
 // 30 us).  With settings of one per row the slowest rows bound the launch, and
 // up to four waves of smaller CTAs even them out (64 x 151643 fp32: 4 CTAs a
-// row 85 us, 8 69 us).
+// row 56 us, 8 51 us, 16 65 us).
 template <class E>
 int launch_split(const SampleArgs& p, int64_t B, cudaStream_t stream) {
   const bool per_row = p.temperature || p.top_k || p.top_p || p.min_p;
@@ -984,7 +1106,7 @@ int launch_split(const SampleArgs& p, int64_t B, cudaStream_t stream) {
   while (c < 8 && c * fit < p.V) c *= 2;
   // Slices that leave room for one CTA per SM only, and more CTAs than SMs: read
   // from L1 and L2 again, so that two CTAs share an SM (64 x 151936 fp32 top-k 50:
-  // 27 us, staged 35; top-p 0.9: 110 against 123).  Not where every token is
+  // 28 us, staged 36; top-p 0.9: 72 against 86).  Not where every token is
   // weighed and nothing filtered (256 x 32000 fp32: 26 us, staged 24.5).
   const bool filters = per_row || p.top_k0 > 0 || p.top_p0 < 1.f || p.min_p0 > 0.f;
   const int64_t smem = static_cast<int64_t>(sizeof(SampShared)) + (p.V + c - 1) / c * static_cast<int64_t>(sizeof(E)) + 16;

@@ -205,6 +205,44 @@ def test_nuclei_of_every_width(top_p, std):
         check(x, u, top_p=top_p, top_k=V // 2)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("min_p", [0.0, 1e-7], ids=["top_p", "min_p"])
+def test_wide_nuclei_of_many_rows(dtype, min_p):
+    """Rows that are read again from global memory, at rows of every alignment; sampled rows are compared."""
+    B, V = 64, 151643
+    for std, top_p in ((2.0, 0.9), (3.0, 0.98), (1.0, 0.5), (2.0, 0.9999)):
+        x, u = make(B, V, int(10 * std), dtype, std)
+        x[:, V - 999:] = -math.inf
+        token, logprob = sample_tokens(x, u, top_p=top_p, min_p=min_p)
+        for b in (0, 1, 2, 3, 31, 63):
+            check(x[b:b + 1], u[b:b + 1], (token[b:b + 1], logprob[b:b + 1]), top_p=top_p, min_p=min_p)
+
+
+@pytest.mark.parametrize("ties", [2, 300, 5000, 100000])
+def test_nucleus_that_ends_inside_ties(ties):
+    """The cut falls into equal logits: a few of them, more than a list holds, and more than a CTA holds."""
+    V = 151643
+    for seed, (top_p, std) in enumerate(((0.3, 1.0), (0.6, 1.0), (0.85, 0.2))):
+        x, u = make(2, V, seed, std=std)
+        at = torch.randperm(V, generator=torch.Generator().manual_seed(seed))[:ties].cuda()
+        for b in range(2):
+            order = x[b].double().sort(descending=True).values
+            mass = (order - order[0]).exp().cumsum(0)
+            x[b, at] = order[int((mass < top_p * mass[-1]).sum())].float()
+        check(x, u, top_p=top_p)
+        check(x.to(torch.bfloat16), u, top_p=top_p)
+
+
+@pytest.mark.parametrize("temperature", [1e-30, 1e-32, 1e-36])
+def test_temperatures_near_the_smallest_number(temperature):
+    """Steps between the logits of the same order as the temperature."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = -30.0 * torch.rand(3, 5003, generator=g, device="cuda", dtype=torch.float64) * temperature
+    u = torch.rand(3, generator=g, device="cuda")
+    for kw in (dict(), dict(top_p=0.9), dict(top_p=0.9999), dict(top_k=2000), dict(top_k=3000, top_p=0.8)):
+        check(x.float(), u, temperature=temperature, **kw)
+
+
 def test_settings_that_are_not_numbers_take_the_first_token():
     x, u = make(4, 3000, 5)
     nan, one = torch.full((4,), math.nan, device="cuda"), torch.ones(4, device="cuda")
