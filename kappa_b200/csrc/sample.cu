@@ -1103,7 +1103,7 @@ int launch_split(const SampleArgs& p, int64_t B, cudaStream_t stream) {
   while (c > 1 && (c * B > most || p.V / c < 2048)) c /= 2;
   const int64_t fit = std::min<int64_t>(
       65535, (kMaxSmem - 16 - static_cast<int64_t>(sizeof(SampShared))) / static_cast<int64_t>(sizeof(E)));
-  while (c < 8 && c * fit < p.V) c *= 2;
+  while (c < kMaxRanks && c * fit < p.V) c *= 2;
   // Slices that leave room for one CTA per SM only, and more CTAs than SMs: read
   // from L1 and L2 again, so that two CTAs share an SM (64 x 151936 fp32 top-k 50:
   // 28 us, staged 36; top-p 0.9: 72 against 86).  Not where every token is

@@ -123,6 +123,17 @@ def test_large_vocabularies(V):
             check(x, u, **kw)
 
 
+@pytest.mark.parametrize("B", [10, 18, 19, 40])
+def test_batches_of_the_largest_vocabulary(B):
+    """Whatever the batch leaves of the CTAs, the slices of a row fit."""
+    x, u = make(B, 393216, B)
+    for kw in (dict(), dict(top_k=20, top_p=0.9), dict(temperature=torch.full((B,), 0.7, device="cuda"), top_p=0.9)):
+        token, logprob = sample_tokens(x, u, **kw)
+        kw = {name: v[:1] if isinstance(v, torch.Tensor) else v for name, v in kw.items()}
+        for b in (0, B - 1):
+            check(x[b:b + 1], u[b:b + 1], (token[b:b + 1], logprob[b:b + 1]), **kw)
+
+
 @pytest.mark.parametrize("V", [1, 7, 1025, 40000])
 def test_ties(V):
     """All logits equal, two values only, and bf16 steps: the lower ids stay."""
