@@ -542,7 +542,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   // Monotone in v: a subtraction, a product cut to [0, 1], a product rounded
   // down (by adding 2^23).
   const float bin_scale = fminf(1.f / (kBinSpan * temp), 1e30f);
-  const bool linear = temp > 1e-31f;  // below, the last bin's weights need not be 0
+  // Beyond, the bins are wider, down to one, or narrower, and the last one's weights need not be 0.
+  const bool linear = temp > 1e-31f && temp < 1e36f;
   const auto bin_of = [&](float v) -> int {
     const float d = __saturatef((top - v) * bin_scale);
     return static_cast<int>(__float_as_uint(__fmaf_rz(d, static_cast<float>(kBins - 1), 8388608.f)) & (kBins - 1));

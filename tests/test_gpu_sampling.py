@@ -254,6 +254,16 @@ def test_temperatures_near_the_smallest_number(temperature):
         check(x.float(), u, temperature=temperature, **kw)
 
 
+@pytest.mark.parametrize("temperature", [9e35, 2e36, 1e37, 2e37, 3e38])
+def test_temperatures_near_the_largest_number(temperature):
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = 3e38 * (2 * torch.rand(3, 5003, generator=g, device="cuda") - 1)
+    u = torch.rand(3, generator=g, device="cuda")
+    for kw in (dict(), dict(top_p=0.9), dict(top_p=0.9999), dict(top_k=2000), dict(top_k=3000, top_p=0.8), dict(top_p=0.7, min_p=0.01)):
+        check(x, u, temperature=temperature, **kw)
+        check(x.to(torch.bfloat16), u, temperature=temperature, **kw)
+
+
 def test_settings_that_are_not_numbers_take_the_first_token():
     x, u = make(4, 3000, 5)
     nan, one = torch.full((4,), math.nan, device="cuda"), torch.ones(4, device="cuda")
