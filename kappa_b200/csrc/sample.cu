@@ -364,9 +364,11 @@ struct Row {
   // (the chord) and to at least e^(-(b + 1/2) s) (c - (S - c / 2) s) (the tangent in
   // the middle), 0.024% less; without S 3% lie between its ends.  Besides, positions
   // are rounded down to 2^-10 bins and weights to whole numbers, and 3 roundings of
-  // 2^-24 move a position by at most 0.0002 bins.  sh.first_bin: the first bin that
-  // the cut can lie in, sh.cut_bin: the first that it cannot lie behind (as it was,
-  // where the bounds do not tell).
+  // 2^-24 move a position by at most 0.0002 bins.  The sum down to the cut is
+  // compared with top_p of all and the sum behind it with 1 - top_p of all, which
+  // is the sharper one near 1 (64 x 151936 fp32, top-p 0.9999: 72 us, 165 without).
+  // sh.first_bin, sh.cut_bin: raised to the first bin that the cut can lie in, and
+  // lowered to the first that it cannot lie behind.
   __device__ __forceinline__ void bound_cut(double top_p, bool fine) {
     constexpr int kPer = kBins / kThreads;
     constexpr double kSpan = static_cast<double>(kBinSpan) / (kBins - 1), kMoved = 0.0005;
@@ -386,12 +388,22 @@ struct Row {
       shi += hi[j];
     }
     u64 at_lo = block_prefix(slo, all_lo), at_hi = block_prefix(shi, all_hi);
-    const double least = top_p * static_cast<double>(all_lo) * (1 - 1e-12), most = top_p * static_cast<double>(all_hi) * (1 + 1e-12);
+    const double total_lo = static_cast<double>(all_lo), total_hi = static_cast<double>(all_hi);
+    const double least = top_p * total_lo * (1 - 1e-12), most = top_p * total_hi * (1 + 1e-12);
+    // (1e-14 of all: the roundings where the exact sums are compared with top_p of them.)
+    const double tail_least = (1 - top_p) * total_lo * (1 - 1e-12) - 1e-14 * total_hi;
+    const double tail_most = (1 - top_p) * total_hi * (1 + 1e-12) + 1e-14 * total_hi;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const uint32_t b = threadIdx.x * kPer + j;
-      if (static_cast<double>(at_hi) < least && !(static_cast<double>(at_hi + hi[j]) < least)) sh.first_bin = b;
-      if (static_cast<double>(at_lo) < most && !(static_cast<double>(at_lo + lo[j]) < most)) sh.cut_bin = b;
+      const double from_lo = static_cast<double>(all_lo - at_lo), behind_lo = static_cast<double>(all_lo - at_lo - lo[j]);
+      const double from_hi = static_cast<double>(all_hi - at_hi), behind_hi = static_cast<double>(all_hi - at_hi - hi[j]);
+      if ((static_cast<double>(at_hi) < least && !(static_cast<double>(at_hi + hi[j]) < least)) ||
+          (from_lo > tail_most && !(behind_lo > tail_most)))
+        atomicMax(&sh.first_bin, b);
+      if ((static_cast<double>(at_lo) < most && !(static_cast<double>(at_lo + lo[j]) < most)) ||
+          (from_hi > tail_least && !(behind_hi > tail_least)))
+        atomicMin(&sh.cut_bin, b);
       at_lo += lo[j];
       at_hi += hi[j];
     }
@@ -422,7 +434,13 @@ struct Row {
   }
 };
 
-template <class E, int kThreads, bool kStaged>
+// What is known at the launch of every row's filters.  In a kernel of their own
+// they lose no registers and instructions to the other paths (64 x 151936 fp32,
+// top-k 50: 24.9 us, 28 in the one for any; 1 x 151936 bf16 top-p 0.9: 24.7
+// against 25.3; 256 x 32000 fp32 without filters: 24.1 against 25.7).
+enum Filters { kNone, kTopK, kNoTopK, kAny };
+
+template <class E, int kThreads, bool kStaged, Filters kFilters>
 __global__ void __launch_bounds__(kThreads, 2)
     sample_kernel(const SampleArgs p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -541,9 +559,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   };
   // Monotone in v: a subtraction, a product cut to [0, 1], a product rounded
   // down (by adding 2^23).
-  const float bin_scale = fminf(1.f / (kBinSpan * temp), 1e30f);
-  // Beyond, the bins are wider, down to one, or narrower, and the last one's weights need not be 0.
-  const bool linear = temp > 1e-31f && temp < 1e36f;
+  // At temperatures that reach the most, bins are narrower, and the last one's weights need not be 0.
+  constexpr float kMostScale = 1e30f;
+  const float bin_scale = fminf(1.f / (kBinSpan * temp), kMostScale);
   const auto bin_of = [&](float v) -> int {
     const float d = __saturatef((top - v) * bin_scale);
     return static_cast<int>(__float_as_uint(__fmaf_rz(d, static_cast<float>(kBins - 1), 8388608.f)) & (kBins - 1));
@@ -556,9 +574,11 @@ __global__ void __launch_bounds__(kThreads, 2)
   const auto upper = [&](float at) { return key_value(min(edge_key(at) + 2, 0xFF800000u)); };
   const auto lower = [&](float at) { return key_value(max(edge_key(at), 0x00800001u) - 2); };
 
-  const bool use_k = k > 0 && k < p.V, use_p = top_p < 1.f, use_m = min_p > 0.f;
+  const bool use_k = kFilters == kTopK || (kFilters == kAny && k > 0 && k < p.V);
+  const bool use_p = kFilters != kNone && top_p < 1.f, use_m = kFilters != kNone && min_p > 0.f;
   // w >= min_p 2^44 in whole numbers (the product is exact).
   const u64 least = use_m ? static_cast<u64>(ceil(static_cast<double>(min_p) * kOne)) : 0;
+  const auto enough = [&](u64 w) { return !use_m || w >= least; };
   const double u = fmin(fmax(static_cast<double>(p.u[row]), 0.0), 1.0);
 
   // For sums in the order of the vocabulary each thread owns a run of
@@ -660,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       __syncthreads();
       if (use_k) {
         R.find_cut(false, static_cast<u64>(k), 0.0, 0);
-      } else if (linear) {
+      } else if (bin_scale < kMostScale && bin_scale > 2e-38f) {  // below, the scale loses bits, and is 0 in the end
         R.bound_cut(static_cast<double>(top_p), fine);
         if (sh.first_bin > 0) run_top = upper(static_cast<float>(sh.first_bin) - 0.5f);
       }
@@ -684,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         sum = R.reduce(sum, add64);
       } else {
         const int window_end = static_cast<int>(sh.cut_bin);
-        const float window_low = linear ? lower(static_cast<float>(window_end) + 1.5f) : -INFINITY;
+        const float window_low = bin_scale < kMostScale ? lower(static_cast<float>(window_end) + 1.5f) : -INFINITY;
         uint32_t lo = 0xffffffffu, hi = 0;
         over_run([&](float v, int i) {
           const u64 w = weight(v);
@@ -786,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         before = R.block_prefix(wp, total);
         const double goal_p = mass ? thr : static_cast<double>(top_p) * static_cast<double>(total);
         const bool keep = tid == 0 || (tid < limit && (!use_p || static_cast<double>(before) < goal_p) &&
-                                       wp >= least);
+                                       enough(wp));
         // The kept ones are the first places: their number, and their sum.
         const u64 both = R.block_reduce(keep ? before + wp : 0, max64);
         total = both;
@@ -831,7 +851,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int j = 0; j < kPer; ++j) {
         const int i = tid * kPer + j;
         const bool keep =
-            i == 0 || (i < limit && (!use_p || static_cast<double>(before) < goal_p) && w[j] >= least);
+            i == 0 || (i < limit && (!use_p || static_cast<double>(before) < goal_p) && enough(w[j]));
         before += w[j];
         if (!keep) w[j] = 0;
         kept += keep;
@@ -952,7 +972,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       R.find_cut(false, static_cast<u64>(k), 0.0, 0);
     }
     // In the last bin every weight is 0: whatever is kept of it is never drawn.
-    if (listed || ((use_k || use_p) && (sh.cut_bin < kBins - 1 || !linear))) refine(mass, static_cast<u64>(k), thr);
+    if (listed || ((use_k || use_p) && (sh.cut_bin < kBins - 1 || bin_scale == kMostScale))) refine(mass, static_cast<u64>(k), thr);
     if (use_k && use_p) {
       R.clear(true);
       u64 s = 0;
@@ -1018,7 +1038,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (v < cut_v || (summed && v > run_top)) continue;
       if (v == cut_v && tie++ >= cut_ties) continue;
       const u64 w = weight(v);
-      if (w >= least) mine += w;
+      if (enough(w)) mine += w;
     }
   }
   const u64 at = R.prefix(mine, total);
@@ -1036,7 +1056,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const bool out = i + lane >= w1 || key < cut_key ||
                        (key == cut_key && tie + __popc(ties & ((1u << lane) - 1)) >= cut_ties);
       u64 w = out ? 0 : weight(v);
-      if (w < least) w = 0;
+      if (!enough(w)) w = 0;
       u64 inc = w;
 #pragma unroll
       for (int s = 1; s < 32; s <<= 1) {
@@ -1058,15 +1078,15 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (ranks > 1) cluster_sync_all();  // no CTA leaves while another reads its shared memory
 }
 
-template <class E, int kThreads, bool kStaged>
+template <class E, int kThreads, bool kStaged, Filters kFilters>
 int launch_typed(SampleArgs p, int64_t B, int64_t c, cudaStream_t stream) {
   int dev = 0;
   KW8_CUDA_TRY(cudaGetDevice(&dev));
   static std::atomic<uint64_t> attr_set{0};
   const uint64_t bit = 1ull << (dev & 63);
   if (!(attr_set.load() & bit)) {
-    KW8_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<E, kThreads, kStaged>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
-    KW8_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<E, kThreads, kStaged>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    KW8_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<E, kThreads, kStaged, kFilters>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
+    KW8_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<E, kThreads, kStaged, kFilters>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     attr_set.fetch_or(bit);
   }
   p.slice = static_cast<int>((p.V + c - 1) / c);
@@ -1085,7 +1105,7 @@ int launch_typed(SampleArgs p, int64_t B, int64_t c, cudaStream_t stream) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  KW8_CUDA_TRY(cudaLaunchKernelEx(&cfg, sample_kernel<E, kThreads, kStaged>, p));
+  KW8_CUDA_TRY(cudaLaunchKernelEx(&cfg, sample_kernel<E, kThreads, kStaged, kFilters>, p));
   return KW8_OK;
 }
 
@@ -1107,12 +1127,17 @@ int launch_split(const SampleArgs& p, int64_t B, cudaStream_t stream) {
   while (c < kMaxRanks && c * fit < p.V) c *= 2;
   // Slices that leave room for one CTA per SM only, and more CTAs than SMs: read
   // from L1 and L2 again, so that two CTAs share an SM (64 x 151936 fp32 top-k 50:
-  // 28 us, staged 36; top-p 0.9: 72 against 86).  Not where every token is
-  // weighed and nothing filtered (256 x 32000 fp32: 26 us, staged 24.5).
-  const bool filters = per_row || p.top_k0 > 0 || p.top_p0 < 1.f || p.min_p0 > 0.f;
+  // 25 us, staged 36; top-p 0.9: 72 against 86).  Not where every token is
+  // weighed and nothing filtered (256 x 32000 fp32: 26 us, staged 24).
   const int64_t smem = static_cast<int64_t>(sizeof(SampShared)) + (p.V + c - 1) / c * static_cast<int64_t>(sizeof(E)) + 16;
-  if (smem > 113 * 1024 && c * B > 148 && filters) return launch_typed<E, 512, false>(p, B, c, stream);
-  return launch_typed<E, 512, true>(p, B, c, stream);
+  const bool staged = smem <= 113 * 1024 || c * B <= 148;
+  if (!p.top_k && p.top_k0 > 0 && p.top_k0 < p.V)
+    return staged ? launch_typed<E, 512, true, kTopK>(p, B, c, stream) : launch_typed<E, 512, false, kTopK>(p, B, c, stream);
+  if (!p.top_k && !p.top_p && !p.min_p && !(p.top_p0 < 1.f) && !(p.min_p0 > 0.f))
+    return launch_typed<E, 512, true, kNone>(p, B, c, stream);
+  if (!p.top_k)
+    return staged ? launch_typed<E, 512, true, kNoTopK>(p, B, c, stream) : launch_typed<E, 512, false, kNoTopK>(p, B, c, stream);
+  return staged ? launch_typed<E, 512, true, kAny>(p, B, c, stream) : launch_typed<E, 512, false, kAny>(p, B, c, stream);
 }
 
 }  // namespace
