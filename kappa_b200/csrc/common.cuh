@@ -263,7 +263,17 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
   }
 }
 
-// Every thread of both CTAs of the cluster: arrive and wait.
+// A barrier of the cluster in two halves, for every thread of its CTAs.  Without
+// the release: it says that a CTA has started (its shared memory may be
+// accessed from now on), not that what it wrote is visible.
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Every thread of the cluster's CTAs: arrive and wait.
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
                    : "memory");

@@ -455,6 +455,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int n = max(0, min(p.slice, p.V - first));
   const E* src = static_cast<const E*>(p.logits) + row * p.ld + (n > 0 ? first : 0);
 
+  // The first exchange below stores into the other CTAs, which must have started: their slices' loads lie
+  // between the two halves of this barrier.
+  if (ranks > 1) cluster_arrive_relaxed();
+
   const float temp = p.temperature ? p.temperature[row] : p.temperature0;
   const float top_p = p.top_p ? p.top_p[row] : p.top_p0;
   const float min_p = p.min_p ? p.min_p[row] : p.min_p0;
@@ -511,6 +515,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     else
       return clean<E>(to_float(__ldg(x + i)));
   };
+  if (ranks > 1) {
+    __syncwarp();
+    cluster_wait();
+  }
   // (key, ~index): the largest value, of equals the lowest index.
   const u64 best_all = R.reduce(
       best_at < 0 ? 0 : (static_cast<u64>(order_key(best)) << 32) | (0xffffffffu - static_cast<uint32_t>(first + best_at)),
