@@ -482,10 +482,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kQ8PairThreads, 1)
         __syncwarp();
         acc_phase ^= 1u << ab;
       }
-      if (elected) mma_commit_pair(&drain_bar);  // arrives once every MMA above has completed
+      if (elected) mma_commit_pair(&drain_bar);  // arrives in both CTAs once every MMA above has completed
+      __syncwarp();
+      if (lane == 0) mbar_wait(&drain_bar, 0, nullptr);  // nothing reads or writes this CTA's memory any more
     }
     __syncwarp();
-    if (lane == 0) mbar_wait(&drain_bar, 0, nullptr);  // both CTAs: nothing reads or writes their memory any more
   } else if (warp >= 4) {
     const int q = warp & 3;
     const int half_of = (warp - 4) >> 2;  // which of the boxes: half_of, half_of + 2, ...
@@ -643,6 +644,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kQ8PairThreads, 1)
       acc_phase ^= 1u << ab;
     }
     if (kTma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    // CTA 1 waits for the MMAs here, behind its tiles: from the start, the wait's
+    // limit would cover the whole launch (262144 x 65536 x 151936 takes 2 s) and
+    // report a timeout where everything goes on.
+    if (!leader && warp == 4 && lane == 0) mbar_wait(&drain_bar, 0, nullptr);
     __syncwarp();
   }
 
