@@ -249,9 +249,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       // both CTAs' barriers are done) once this arrives.
       mma_commit_pair(&drain_bar);
       mbar_wait(&drain_bar, 0, nullptr);
-    } else if (lane == 0) {
-      // CTA 1: the pair's last commit also arrives here.
-      mbar_wait(&drain_bar, 0, nullptr);
     }
   } else if (warp >= kTcFirstConvWarp && warp < kTcFirstConvWarp + kTcConvWarps) {
     // ------------------------------------------------------ converters ----
@@ -331,6 +328,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       if (lane == 0) mbar_arrive_cluster(acc_empty0 + 8u * static_cast<uint32_t>(ab));
       acc_phase ^= 1u << ab;
     }
+    // CTA 1: the pair's last commit arrives here too.  Waited for behind the
+    // tiles, so that the wait's limit does not cover the whole launch.
+    if (!leader && warp == kTcFirstEpiWarp && lane == 0) mbar_wait(&drain_bar, 0, nullptr);
+    __syncwarp();
   }
 
   tc_fence_before();
