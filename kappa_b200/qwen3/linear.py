@@ -28,14 +28,18 @@ __all__ = ["project_q", "project_kv", "project_attn_out", "quantize_attn_out", "
            "linear_q8"]
 
 
-def linear_q8(x: Q8Rows, w: Weight, *, in_axis: int = -1, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+def linear_q8(x: Q8Rows, w: Weight | KMajor, *, in_axis: int = -1,
+              out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """8-bit rows ``[.., K]`` times a W8 weight ``[.., N, K]`` (``in_axis=-1``) or ``[.., K, N]`` (``-2``): ``[.., N]``.
 
     ``out[t, n] = (sum_k x.values[t, k] * w.values[n, k]) * x.scale[t] * w.scale[n]``; N counts the leading axes of a
-    stacked weight too.
+    stacked weight too.  A weight that is K-major already (``attn_out_kmajor``'s, for the output projection on heads
+    flattened to ``[.., n * h]``) is taken as it is.
     """
     if not isinstance(x, Q8Rows):
         raise TypeError("x: linear_q8 takes 8-bit rows (add_rms_norm_q8, rms_norm_q8)")
+    if isinstance(w, KMajor):
+        return _dense.linear_q8(x, w, out_dtype=out_dtype)
     if type(w) is Q8Weight and in_axis == -1:
         # A weight [N, K] as it is stored: no views to make (kmajor's take as long as the launch).
         q, s = w
