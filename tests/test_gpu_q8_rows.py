@@ -7,8 +7,9 @@ import torch
 
 from kappa_b200 import _lib
 from kappa_b200.qwen3 import linear as qlin
+from kappa_b200.qwen3 import transformer as QT
 from kappa_b200.qwen3.quant import Q8Rows
-from test_gpu_linear_q8 import _ref, _rows
+from test_gpu_linear_q8 import _ref, _rows, _weight
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +38,40 @@ def test_the_output_projection_on_8_bit_rows(B, T, per_channel):
         qlin.project_attn_out(x3, o)
     with pytest.raises(ValueError, match="features"):
         qlin.linear_q8(Q8Rows(x3.values[..., :-16], x3.scale), qlin.attn_out_kmajor(o))
+
+
+@pytest.mark.parametrize("dtype", [None, torch.float32])
+@pytest.mark.parametrize("B,L", [(1, 1), (3, 7), (40, 5)])
+def test_last_positions_of_8_bit_rows(B, L, dtype):
+    """Positions as JAX's gather takes them: negative ones count from the end, all are clamped."""
+    D, V = 256, 1001
+    x, w = _rows(B * L, D, L), _weight(V, D, 3)
+    x3 = Q8Rows(x.values.reshape(B, L, D), x.scale.reshape(B, L, 1))
+    last = torch.tensor([(3 * i) % (2 * L + 3) - L - 1 for i in range(B)], device="cuda")
+    at = [min(max(int(i) + L if int(i) < 0 else int(i), 0), L - 1) for i in last]
+    rows = torch.arange(B, device="cuda") * L + torch.tensor(at, device="cuda")
+    want = _ref(Q8Rows(x.values[rows], x.scale[rows]), w, dtype or torch.bfloat16)
+    assert torch.equal(QT.logits_from_hidden_last_positions(x3, w, last, out_dtype=dtype), want)
+    strided = Q8Rows(x3.values.transpose(0, 1).contiguous().transpose(0, 1), x3.scale)
+    assert torch.equal(QT.logits_from_hidden_last_positions(strided, w, last, out_dtype=dtype), want)
+
+
+def test_last_positions_refuses():
+    w = _weight(96, 64, 1)
+    for x in (_rows(6, 64, 2), torch.zeros(6, 64, dtype=torch.bfloat16, device="cuda")):
+        def shaped(*s, x=x):
+            return Q8Rows(x.values.reshape(*s), x.scale.reshape(*s[:-1], 1)) if isinstance(x, Q8Rows) else x.reshape(*s)
+
+        def empty(x=x):
+            return Q8Rows(x.values[:0].reshape(2, 0, 64), x.scale[:0].reshape(2, 0, 1)) if isinstance(x, Q8Rows) \
+                else x[:0].reshape(2, 0, 64)
+
+        two = torch.zeros(2, dtype=torch.int64, device="cuda")
+        with pytest.raises(ValueError, match="last_idx"):
+            QT.logits_from_hidden_last_positions(shaped(3, 2, 64), w, two)
+        with pytest.raises(ValueError, match="must be"):
+            QT.logits_from_hidden_last_positions(shaped(6, 64), w, two)
+        with pytest.raises(ValueError):
+            QT.logits_from_hidden_last_positions(shaped(2, 3, 64), _weight(96, 32, 1), two)
+        with pytest.raises(ValueError, match="no positions"):
+            QT.logits_from_hidden_last_positions(empty(), w, two)
