@@ -204,7 +204,17 @@ def kmajor(w: Weight, in_axis: int, name: str = "weight") -> KMajor:
             raise ValueError(f"{name}: packed with contraction axis {w.in_axis}, used with {in_axis}")
         _lib.require_cuda(w.tiled, name)
         s = w.scale
+        # The kernels read it without further checks.
+        if s.dtype not in _DT:
+            raise ValueError(f"{name}: scale dtype {s.dtype} unsupported")
+        if s.device != w.tiled.device:
+            raise ValueError(f"{name}: scale and values on different devices")
         per_channel = s.numel() > 1
+        channels = 1
+        for d in w.kshape[:-1]:
+            channels *= int(d)
+        if s.numel() != 1 and s.numel() != channels:
+            raise ValueError(f"{name}: scale has {s.numel()} values, expected 1 or {channels}")
         s = s.contiguous().reshape(-1) if per_channel else s.reshape(1).contiguous()
         return KMajor(q=w.tiled, scale=s, per_channel=per_channel, shape=tuple(int(d) for d in w.kshape),
                       layout=_lib.LAYOUT_TILED)

@@ -8,7 +8,7 @@ import torch
 from kappa_b200 import _lib
 from kappa_b200.qwen3 import linear as qlin
 from kappa_b200.qwen3 import transformer as QT
-from kappa_b200.qwen3.quant import Q8Rows
+from kappa_b200.qwen3.quant import Q8Rows, kmajor, pack_weight
 from test_gpu_linear_q8 import _ref, _rows, _weight
 
 pytestmark = pytest.mark.gpu
@@ -75,3 +75,16 @@ def test_last_positions_refuses():
             QT.logits_from_hidden_last_positions(shaped(2, 3, 64), _weight(96, 32, 1), two)
         with pytest.raises(ValueError, match="no positions"):
             QT.logits_from_hidden_last_positions(empty(), w, two)
+
+
+def test_a_packed_weight_brings_a_scale_that_fits():
+    """Refused as a K-major weight's is, before anything reads it."""
+    w = pack_weight(_weight(48, 64, 1), in_axis=-1)
+    for scale, text in ((w.scale.cpu(), "devices"), (w.scale.half(), "dtype"), (w.scale[:-1], "expected 1 or 48"),
+                        (torch.cat([w.scale, w.scale]), "expected 1 or 48"), (w.scale[:0], "expected 1 or 48")):
+        with pytest.raises(ValueError, match=text):
+            kmajor(w._replace(scale=scale), -1)
+    x = _rows(3, 64, 2)
+    with pytest.raises(ValueError, match="devices"):
+        qlin.linear_q8(x, w._replace(scale=w.scale.cpu()))
+    assert torch.equal(qlin.linear_q8(x, w), _ref(x, _weight(48, 64, 1), torch.bfloat16))
