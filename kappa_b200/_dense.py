@@ -125,8 +125,8 @@ def linear_q8_rows(x: Q8Rows, w: _lib.KW8Weight, wq: torch.Tensor, N: int, K: in
     if vc.data_ptr() % 16:
         vc = vc.clone()
     out = vc.new_empty(shape[:-1] + (N,), dtype=out_dtype)
-    code = _lib.load().kw8_linear_q8(vc.data_ptr(), sc.data_ptr(), vc.numel() // K, K, N, w, dt, out.data_ptr(),
-                                     _lib.stream_of(vc))
+    code = _lib.load().kw8_linear_q8(vc.data_ptr(), sc.data_ptr(), vc.numel() // K if K else 0, K, N, w, dt,
+                                     out.data_ptr(), _lib.stream_of(vc))
     if code:
         _lib.check(code)
     return out

@@ -8,7 +8,7 @@ import torch
 from kappa_b200 import _lib
 from kappa_b200.qwen3 import linear as qlin
 from kappa_b200.qwen3 import transformer as QT
-from kappa_b200.qwen3.quant import Q8Rows, kmajor, pack_weight
+from kappa_b200.qwen3.quant import Q8Rows, Q8Weight, kmajor, pack_weight
 from test_gpu_linear_q8 import _ref, _rows, _weight
 
 pytestmark = pytest.mark.gpu
@@ -88,3 +88,12 @@ def test_a_packed_weight_brings_a_scale_that_fits():
     with pytest.raises(ValueError, match="devices"):
         qlin.linear_q8(x, w._replace(scale=w.scale.cpu()))
     assert torch.equal(qlin.linear_q8(x, w), _ref(x, _weight(48, 64, 1), torch.bfloat16))
+
+
+@pytest.mark.parametrize("N,K", [(32, 0), (0, 64), (0, 0)])
+@pytest.mark.parametrize("T", [0, 4])
+def test_weights_without_rows_or_features_are_refused(T, N, K):
+    x = Q8Rows(torch.zeros(T, K, dtype=torch.int8, device="cuda"), torch.ones(T, 1, device="cuda"))
+    w = Q8Weight(torch.zeros(N, K, dtype=torch.int8, device="cuda"), torch.ones((), device="cuda"))
+    with pytest.raises(ValueError, match="bad shape"):
+        qlin.linear_q8(x, w)
