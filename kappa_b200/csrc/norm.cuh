@@ -29,7 +29,7 @@ int launch_block_finish(const float* part, int splits, int64_t split_stride, int
 //   h = residual ? bf16(f32(x) + f32(residual)) : x     (stored to h_out if given)
 //   y = (f32(h) * rsqrt(mean(f32(h)^2) + eps)) * g      (fp32)
 //   q_out == nullptr:  y_out = bf16(y)
-//   else:  s = max(max|y| / 127, FLT_MIN),  q_out = round_half_even(y / s),  s_out[row] = s.
+//   else:  s = max(max|y| / 127, FLT_MIN),  q_out = round_half_even(y * (1 / s)),  s_out[row] = s.
 // A row whose y is not finite gets q = 0 and s = NaN.  h_out may be x or
 // residual (in place); otherwise the outputs overlap nothing.
 int launch_add_rms_norm(const void* x, const void* residual, int64_t T, int64_t D, const void* scale,

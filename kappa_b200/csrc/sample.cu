@@ -14,8 +14,9 @@
 // result is the same for every split of a row.  A token below 2^-44 of the
 // most likely one has weight 0.
 //
-// A cluster of up to eight CTAs takes a row; each holds its slice in shared
-// memory, so the logits are read once.  Every filter cuts the same order, so a
+// A cluster of up to sixteen CTAs takes a row; each holds its slice in shared
+// memory, so the logits are read once (slices that leave no room for a second
+// CTA on the SM are read from L1 and L2 again).  Every filter cuts the same order, so a
 // histogram of kBins bins linear in (m - x) / temperature (a monotone function)
 // finds the bin of each cut.  Then, with M the tokens down to that bin:
 //   M <= kList: one CTA collects, sorts and finishes them (the usual settings);
@@ -27,6 +28,8 @@
 //   top-p 0.9: 72 us, 110 through all tokens).
 // CTAs add their histograms through distributed shared memory.
 #include "sample.cuh"
+
+#include "gemm_tc.cuh"
 
 #include <cmath>
 
@@ -567,7 +570,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   };
   // Monotone in v: a subtraction, a product cut to [0, 1], a product rounded
   // down (by adding 2^23).
-  // At temperatures that reach the most, bins are narrower, and the last one's weights need not be 0.
+  // At temperatures below 1 / (32 kMostScale) the bins are wider than that; the last one begins further than
+  // kBinSpan e-folds from the maximum, so its weights are 0 all the same.
   constexpr float kMostScale = 1e30f;
   const float bin_scale = fminf(1.f / (kBinSpan * temp), kMostScale);
   const auto bin_of = [&](float v) -> int {
@@ -688,7 +692,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       __syncthreads();
       if (use_k) {
         R.find_cut(false, static_cast<u64>(k), 0.0, 0);
-      } else if (bin_scale < kMostScale && bin_scale > 2e-38f) {  // below, the scale loses bits, and is 0 in the end
+      } else if (bin_scale < kMostScale && bin_scale > 2e-38f) {  // bins of the width that bound_cut() takes them for:
+        // wider at the most, and below 2e-38 the scale loses bits, and is 0 in the end
         R.bound_cut(static_cast<double>(top_p), fine);
         if (sh.first_bin > 0) run_top = upper(static_cast<float>(sh.first_bin) - 0.5f);
       }
@@ -712,7 +717,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         sum = R.reduce(sum, add64);
       } else {
         const int window_end = static_cast<int>(sh.cut_bin);
-        const float window_low = bin_scale < kMostScale ? lower(static_cast<float>(window_end) + 1.5f) : -INFINITY;
+        const float window_low = lower(static_cast<float>(window_end) + 1.5f);
         uint32_t lo = 0xffffffffu, hi = 0;
         over_run([&](float v, int i) {
           const u64 w = weight(v);
@@ -980,7 +985,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       R.find_cut(false, static_cast<u64>(k), 0.0, 0);
     }
     // In the last bin every weight is 0: whatever is kept of it is never drawn.
-    if (listed || ((use_k || use_p) && (sh.cut_bin < kBins - 1 || bin_scale == kMostScale))) refine(mass, static_cast<u64>(k), thr);
+    if (listed || ((use_k || use_p) && sh.cut_bin < kBins - 1)) refine(mass, static_cast<u64>(k), thr);
     if (use_k && use_p) {
       R.clear(true);
       u64 s = 0;
@@ -1087,9 +1092,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 template <class E, int kThreads, bool kStaged, Filters kFilters>
-int launch_typed(SampleArgs p, int64_t B, int64_t c, cudaStream_t stream) {
-  int dev = 0;
-  KW8_CUDA_TRY(cudaGetDevice(&dev));
+int launch_typed(SampleArgs p, int64_t B, int64_t c, int dev, cudaStream_t stream) {
   static std::atomic<uint64_t> attr_set{0};
   const uint64_t bit = 1ull << (dev & 63);
   if (!(attr_set.load() & bit)) {
@@ -1126,26 +1129,30 @@ int launch_typed(SampleArgs p, int64_t B, int64_t c, cudaStream_t stream) {
 // row 56 us, 8 51 us, 16 65 us).
 template <class E>
 int launch_split(const SampleArgs& p, int64_t B, cudaStream_t stream) {
+  int dev = 0;
+  KW8_CUDA_TRY(cudaGetDevice(&dev));
+  const int64_t sms = num_sms(dev);
   const bool per_row = p.temperature || p.top_k || p.top_p || p.min_p;
-  const int64_t most = per_row ? 4 * 148 : 148;
+  const int64_t most = per_row ? 4 * sms : sms;
   int64_t c = per_row ? 8 : 16;
   while (c > 1 && (c * B > most || p.V / c < 2048)) c /= 2;
-  const int64_t fit = std::min<int64_t>(
+  constexpr int64_t fit = std::min<int64_t>(
       65535, (kMaxSmem - 16 - static_cast<int64_t>(sizeof(SampShared))) / static_cast<int64_t>(sizeof(E)));
+  static_assert(kMaxRanks * fit >= kSampleMaxV, "the largest vocabulary must fit into a cluster's shared memory");
   while (c < kMaxRanks && c * fit < p.V) c *= 2;
   // Slices that leave room for one CTA per SM only, and more CTAs than SMs: read
   // from L1 and L2 again, so that two CTAs share an SM (64 x 151936 fp32 top-k 50:
   // 25 us, staged 36; top-p 0.9: 72 against 86).  Not where every token is
   // weighed and nothing filtered (256 x 32000 fp32: 26 us, staged 24).
   const int64_t smem = static_cast<int64_t>(sizeof(SampShared)) + (p.V + c - 1) / c * static_cast<int64_t>(sizeof(E)) + 16;
-  const bool staged = smem <= 113 * 1024 || c * B <= 148;
+  const bool staged = smem <= 113 * 1024 || c * B <= sms;
   if (!p.top_k && p.top_k0 > 0 && p.top_k0 < p.V)
-    return staged ? launch_typed<E, 512, true, kTopK>(p, B, c, stream) : launch_typed<E, 512, false, kTopK>(p, B, c, stream);
+    return staged ? launch_typed<E, 512, true, kTopK>(p, B, c, dev, stream) : launch_typed<E, 512, false, kTopK>(p, B, c, dev, stream);
   if (!p.top_k && !p.top_p && !p.min_p && !(p.top_p0 < 1.f) && !(p.min_p0 > 0.f))
-    return launch_typed<E, 512, true, kNone>(p, B, c, stream);
+    return launch_typed<E, 512, true, kNone>(p, B, c, dev, stream);
   if (!p.top_k)
-    return staged ? launch_typed<E, 512, true, kNoTopK>(p, B, c, stream) : launch_typed<E, 512, false, kNoTopK>(p, B, c, stream);
-  return staged ? launch_typed<E, 512, true, kAny>(p, B, c, stream) : launch_typed<E, 512, false, kAny>(p, B, c, stream);
+    return staged ? launch_typed<E, 512, true, kNoTopK>(p, B, c, dev, stream) : launch_typed<E, 512, false, kNoTopK>(p, B, c, dev, stream);
+  return staged ? launch_typed<E, 512, true, kAny>(p, B, c, dev, stream) : launch_typed<E, 512, false, kAny>(p, B, c, dev, stream);
 }
 
 }  // namespace

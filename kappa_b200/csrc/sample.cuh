@@ -5,7 +5,7 @@
 
 namespace kw8 {
 
-constexpr int64_t kSampleMaxV = 8 * 49152;  // eight CTAs' shared memory of fp32 logits
+constexpr int64_t kSampleMaxV = 8 * 49152;  // sixteen CTAs' shared memory holds it in fp32, eight nearly (387360)
 
 struct SampleArgs {
   const void* logits;  // row r at logits + r * ld
