@@ -6,10 +6,12 @@ import pytest
 import torch
 
 from kappa_b200 import _lib
+from kappa_b200.gemma3 import norms
 from kappa_b200.qwen3 import linear as qlin
 from kappa_b200.qwen3 import transformer as QT
 from kappa_b200.qwen3.quant import Q8Rows, Q8Weight, kmajor, pack_weight
 from test_gpu_linear_q8 import _ref, _rows, _weight
+from test_gpu_norm_q8 import _norm64
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +99,28 @@ def test_weights_without_rows_or_features_are_refused(T, N, K):
     w = Q8Weight(torch.zeros(N, K, dtype=torch.int8, device="cuda"), torch.ones((), device="cuda"))
     with pytest.raises(ValueError, match="bad shape"):
         qlin.linear_q8(x, w)
+
+
+@pytest.mark.parametrize("loud", [0.0, 20.0, 100.0])
+def test_what_8_bit_rows_cost_in_accuracy(loud):
+    """The norm's rows in 8 bits, multiplied, against the product of the rows in 64 bits.
+
+    A value of a row is off by at most half a step and what test_gpu_norm_q8.py derives (2^-8 steps, and 127 * 2^-17 for
+    the scale): below 0.505 steps of max|y| / 127, whatever its own size.  So features that are far larger than the others
+    cost the others their accuracy, and an output is off by at most 0.505 max|y| / 127 times the sum of its weights'
+    sizes (and three fp32 roundings).  The bound is kept to; the rows of loud features do cost.
+    """
+    g = torch.Generator(device="cuda").manual_seed(1)
+    T, D, N = 64, 1024, 512
+    m = 1 + loud * (torch.rand(D, generator=g, device="cuda") < 0.004)
+    x = (torch.randn(T, D, generator=g, device="cuda") * m).to(torch.bfloat16)
+    r = (3 * torch.randn(T, D, generator=g, device="cuda") * m).to(torch.bfloat16)
+    gain = 0.1 * torch.randn(D, generator=g, device="cuda")
+    w = _weight(N, D, 5)
+    h, q = norms.add_rms_norm_q8(x, r, gain)
+    y = _norm64(h, gain, True)
+    ws = w.values.double() * w.scale.double()
+    want = y @ ws.t()
+    step = y.abs().amax(-1, keepdim=True) / 127
+    far = (qlin.linear_q8(q, w, out_dtype=torch.float32).double() - want).abs()
+    assert (far <= 0.505 * step * ws.abs().sum(-1) + 2.0 ** -22 * want.abs()).all()
