@@ -645,7 +645,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kQ8PairThreads, 1)
     }
     if (kTma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     // CTA 1 waits for the MMAs here, behind its tiles: from the start, the wait's
-    // limit would cover the whole launch (262144 x 65536 x 151936 takes 2 s) and
+    // limit would cover the whole launch (180224 x 131056 x 180224 takes more) and
     // report a timeout where everything goes on.
     if (!leader && warp == 4 && lane == 0) mbar_wait(&drain_bar, 0, nullptr);
     __syncwarp();
@@ -668,8 +668,12 @@ int q8_cols(int nt) {
 
 // The choice between the two kernels, their tiles and the K splits is the least
 // of these models (us beyond a common part), fitted to 657 shapes of 17 to 1000
-// rows, K 64 to 9728 and 64 to 40960 channels: 1.8% above the best of the
-// measured choices on average, 31% at worst.  Both sides of it: 96 x 2048 x 4096
+// rows, K 64 to 9728 and 64 to 40960 channels: 1.9% above the best of the
+// measured choices on average, more than 10% at 49 of them, 31% at worst (33 to 64
+// rows of 9728 x 20480: 32-row tiles 51 us, the best 39 to 40).  Outside of that,
+// measured afterwards: heads of 151936 channels, 1 to 300 rows, K 1024 to 2560: always
+// the best; 1500 to 8192 rows, K 64 to 4096, 64 to 8192 channels: 1.2% above it on
+// average, 25% at worst (8192 x 64 x 64: 6.3 us, pairs 5.0).  Both sides of it: 96 x 2048 x 4096
 // 8.4 us here, 7.3 with pairs; 77 x 2560 x 10243 11 us, 12.7 with pairs; 256 x 9728
 // x 64 8 us, 15 with pairs; 64 x 2048 x 151936 66 us with 64-row tiles, 74 with
 // 32-row ones, 69 with pairs.
